@@ -306,6 +306,76 @@ int kx_conv2d_backward_f64(kx_handle *h, const kx_tensor *input, const kx_tensor
                            const kx_conv2d_options *options, const kx_tensor *grad_input,
                            const kx_tensor *grad_weight, kx_error *err);
 
+/* ---- from logits to an update -------------------------------------------- */
+/* No counterparts in the reference, which has softmax (above) for the first
+ * and Tape's products (above) on either side of them.  All four are ordered on
+ * the handle's stream, read nothing back, allocate nothing and can be captured
+ * into a CUDA graph.  `tokens` and `top_tokens` hold int64 elements.
+ *
+ * Log probabilities of given tokens: over the last axis of `logits` (any
+ * strides, 1 <= rank), with z = logits / temperature,
+ *   lse       = log sum exp z,
+ *   log_probs = z[token] - lse, one token for each row,
+ *   entropy   = -sum p log p with p = exp(z - lse),
+ *   top_*     = the largest logits' z - lse and their places, in falling order,
+ *               the lower place first among equal ones.
+ * `tokens` (any strides), `log_probs`, `lse` and `entropy` have logits' dims
+ * without the last; `top_log_probs` and `top_tokens` have a last axis of 0 to
+ * 32 alternatives instead.  Each output is C-contiguous and may be NULL, but
+ * not all; tokens goes with log_probs, top_log_probs with top_tokens.
+ * A logit of -inf is a token taken out by a mask: it has probability 0 and log
+ * probability -inf, and is no alternative.  Alternatives that a row does not
+ * have are -inf with token -1; a row whose mask leaves nothing has an lse and
+ * log probability of -inf and an entropy of 0.  A token below 0 stands for a
+ * position without one: its log probability is 0.  A token at or above the
+ * vocabulary gives NaN, and a row that holds a NaN or +inf gives NaN in each
+ * output, with -1 for its alternatives' tokens (nothing is raised: the values
+ * are never read by the host).  KX_E_PARAM names a temperature that is not
+ * finite and > 0 (or whose reciprocal is not), before everything else. */
+int kx_token_log_probs_f32(kx_handle *h, const kx_tensor *logits, const kx_tensor *tokens, float temperature,
+                           const kx_tensor *log_probs, const kx_tensor *lse, const kx_tensor *entropy,
+                           const kx_tensor *top_log_probs, const kx_tensor *top_tokens, kx_error *err);
+int kx_token_log_probs_f64(kx_handle *h, const kx_tensor *logits, const kx_tensor *tokens, double temperature,
+                           const kx_tensor *log_probs, const kx_tensor *lse, const kx_tensor *entropy,
+                           const kx_tensor *top_log_probs, const kx_tensor *top_tokens, kx_error *err);
+/* Their gradient: grad_logits (C-contiguous, logits' dims) =
+ *   [p (grad_lse - grad_log_probs - grad_entropy (log p + entropy))
+ *    + grad_log_probs at the token] / temperature,
+ * 0 for a logit of -inf.  Each of the three incoming gradients (one for each
+ * row, any strides) may be NULL, but not all.  `lse` and, with grad_entropy,
+ * `entropy` are the forward call's for these logits and this temperature;
+ * `tokens` goes with grad_log_probs.  A token below 0 takes no part of
+ * grad_log_probs; one at or above the vocabulary gives its row NaN, as do NaN
+ * and +inf among its logits. */
+int kx_token_log_probs_backward_f32(kx_handle *h, const kx_tensor *logits, const kx_tensor *tokens,
+                                    const kx_tensor *lse, const kx_tensor *entropy, const kx_tensor *grad_log_probs,
+                                    const kx_tensor *grad_entropy, const kx_tensor *grad_lse, float temperature,
+                                    const kx_tensor *grad_logits, kx_error *err);
+int kx_token_log_probs_backward_f64(kx_handle *h, const kx_tensor *logits, const kx_tensor *tokens,
+                                    const kx_tensor *lse, const kx_tensor *entropy, const kx_tensor *grad_log_probs,
+                                    const kx_tensor *grad_entropy, const kx_tensor *grad_lse, double temperature,
+                                    const kx_tensor *grad_logits, kx_error *err);
+/* The 2-norm over all elements of `count` gradients (0 to 2^24 of them, any
+ * dims and strides) into the one element of `norm`, its squares added in 64
+ * bits in a fixed order.  `workspace` is the caller's device memory, 8-byte
+ * aligned, of at least the bytes that kx_grad_norm_workspace (host only)
+ * gives; two calls that may run at the same time need one each. */
+int kx_grad_norm_workspace(uint64_t count, uint64_t *bytes);
+int kx_grad_norm_f32(kx_handle *h, const kx_tensor *grads, uint64_t count, const kx_tensor *norm, void *workspace,
+                     uint64_t workspace_bytes, kx_error *err);
+int kx_grad_norm_f64(kx_handle *h, const kx_tensor *grads, uint64_t count, const kx_tensor *norm, void *workspace,
+                     uint64_t workspace_bytes, kx_error *err);
+/* The same norm, and outs[i] = grads[i] * min(1, max_norm / norm).  Each
+ * output has its gradient's dims and any strides that give each element a
+ * place of its own (else KX_E_ALIAS); it may be its gradient itself (same
+ * data, origin and strides), and its span overlaps no other operand
+ * (KX_E_ALIAS).  With a norm of at most max_norm, or one that is not finite,
+ * the outputs are the gradients as they were.  max_norm is finite and > 0. */
+int kx_clip_grad_norm_f32(kx_handle *h, const kx_tensor *grads, uint64_t count, double max_norm, const kx_tensor *outs,
+                          const kx_tensor *norm, void *workspace, uint64_t workspace_bytes, kx_error *err);
+int kx_clip_grad_norm_f64(kx_handle *h, const kx_tensor *grads, uint64_t count, double max_norm, const kx_tensor *outs,
+                          const kx_tensor *norm, void *workspace, uint64_t workspace_bytes, kx_error *err);
+
 /* ---- host-buffer hooks (MatmulElement) ---------------------------------- */
 /* try_dense_matmul: C-order a[m*k], b[k*n] -> out[m*n] in HOST memory.
  * Returns KX_DECLINED (nothing written) on any length mismatch, exactly like

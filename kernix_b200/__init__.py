@@ -7,6 +7,8 @@ The public names follow the reference crate (kernix-ops):
 * ``softmax_temperature(s, axis, t)`` ops/math_extra.rs:544-557
 * ``softmax(s, axis)``             ops/math.rs:531-536
 * ``attention(q, kt, v, t)``       matmul + softmax_temperature + matmul in one call
+* ``token_log_probs(logits, tokens)`` and its gradient, ``grad_norm(grads)``,
+  ``clip_grad_norm(grads, max)``    from logits to an update
 * ``MatrixInput`` / ``try_dense_matmul`` / ``try_strided_matmul``
                                    ops/matmul_element.rs:14-44, 262-300
 * ``CudaExecutor``                 the ``MatmulDevice`` / ``Device`` plug point
@@ -23,7 +25,7 @@ import contextlib
 import ctypes as C
 import threading
 from dataclasses import dataclass, field
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import numpy as np
 
@@ -40,6 +42,8 @@ MAX_RANK = _abi.MAX_RANK
 __all__ = [
     "matmul", "matmul_reference", "matmul_shape", "matmul_into", "conv2d", "conv2d_reference", "conv2d_shape",
     "Conv2dOptions", "attention", "attention_into", "matmul_backward", "conv2d_backward", "tensordot", "softmax", "softmax_into", "softmax_temperature", "matmul_into_replicated", "conv2d_into", "softmax_temperature_into",
+    "token_log_probs", "token_log_probs_into", "token_log_probs_backward", "token_log_probs_backward_into",
+    "TokenLogProbs", "grad_norm", "grad_norm_into", "clip_grad_norm", "clip_grad_norm_into",
     "MatrixInput", "try_dense_matmul", "try_strided_matmul", "TensorView", "CudaExecutor", "Handle",
     "handle", "OpsError", "InvalidRank", "ContractDimensionMismatch", "BroadcastIncompatible",
     "ElementCountOverflow", "DimensionOverflow", "LayoutError", "InvalidParameter", "ExactRank",
@@ -507,6 +511,212 @@ def softmax_into(src, axis: int, out) -> None:
     err = KxError()
     ds, do = _descriptor(src), _descriptor(out)
     raise_for(fn(h.ptr, C.byref(ds), int(axis), C.byref(do), C.byref(err)), err)
+
+
+# ---------------------------------------------------------------------------
+# from logits to an update
+# ---------------------------------------------------------------------------
+MAX_ALTERNATIVES = 32
+
+
+class TokenLogProbs(NamedTuple):
+    """What ``token_log_probs`` gives for each row of logits; None for what was
+    not asked for."""
+
+    log_probs: "object" = None          # of the given token
+    lse: "object" = None                # log sum exp of logits / temperature
+    entropy: "object" = None
+    top_log_probs: "object" = None      # [.., top], falling
+    top_tokens: "object" = None         # [.., top], int64
+
+
+def _same_device(op: str, dev: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and _device_index(t) != dev:
+            raise InvalidParameter(f"{op}: {name} belongs to another device", operation=op, parameter=name)
+
+
+def _same_dtype(op: str, dtype, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.dtype != dtype:
+            raise InvalidParameter(f"{op}: {name} is {t.dtype}, not {dtype}", operation=op, parameter=name)
+
+
+def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int = 0,
+                    entropy: bool = False) -> TokenLogProbs:
+    """Log probabilities of given tokens under ``softmax(logits / temperature)``
+    along the last axis, with the log-sum-exp of each row and, if asked for,
+    its ``entropy`` and the ``top`` (at most 32) likeliest tokens, in one pass
+    over the logits.
+
+    ``tokens`` (int64) has logits' dims without the last; without it no
+    ``log_probs`` come back.  A token below 0 stands for a position that has
+    none (log probability 0).  Logits of -inf are masked tokens: probability 0,
+    never an alternative (a row that runs out of them has -inf and token -1); a
+    row whose mask leaves nothing has lse and log probability -inf and entropy
+    0.  A token at or above the vocabulary, or a row with a NaN or +inf, gives
+    NaN instead of raising: nothing is read back, so the call does not wait for
+    the device and can be captured into a CUDA graph."""
+    import torch
+    shape = tuple(logits.shape)
+    top = int(top)
+    if not 0 <= top <= MAX_ALTERNATIVES:
+        raise InvalidParameter(f"token_log_probs: top (0 to {MAX_ALTERNATIVES} alternatives)",
+                               operation="token_log_probs", parameter="top")
+    rows = shape[:-1]
+    make = lambda dims, dtype: torch.empty(dims, dtype=dtype, device=logits.device)  # noqa: E731
+    out = TokenLogProbs(
+        log_probs=make(rows, logits.dtype) if tokens is not None else None,
+        lse=make(rows, logits.dtype),
+        entropy=make(rows, logits.dtype) if entropy else None,
+        top_log_probs=make((*rows, top), logits.dtype) if top else None,
+        top_tokens=make((*rows, top), torch.int64) if top else None)
+    token_log_probs_into(logits, tokens, out, temperature=temperature)
+    return out
+
+
+def token_log_probs_into(logits, tokens, out: TokenLogProbs, *, temperature: float = 1.0) -> None:
+    """``token_log_probs`` written into existing C-contiguous tensors; those
+    that ``out`` holds decide what is computed."""
+    import torch
+    op = "token_log_probs"
+    fn = _fn("kx_token_log_probs", logits.dtype)
+    h = _bind(logits)
+    _same_device(op, h.device, tokens=tokens, **out._asdict())
+    _same_dtype(op, logits.dtype, log_probs=out.log_probs, lse=out.lse, entropy=out.entropy,
+                top_log_probs=out.top_log_probs)
+    _same_dtype(op, torch.int64, tokens=tokens, top_tokens=out.top_tokens)
+    err = KxError()
+    dl, dt = _ref(logits), _ref(tokens)
+    raise_for(fn(h.ptr, dl, dt, float(temperature), *[_ref(t) for t in out], C.byref(err)), err)
+
+
+def _ref(t):
+    return None if t is None else C.byref(_descriptor(t))
+
+
+def token_log_probs_backward(logits, tokens=None, *, lse, entropy=None, grad_log_probs=None, grad_entropy=None,
+                             grad_lse=None, temperature: float = 1.0):
+    """The gradient with respect to ``logits`` of ``token_log_probs``' outputs:
+    ``[p (grad_lse - grad_log_probs - grad_entropy (log p + entropy)) +
+    grad_log_probs at the token] / temperature``, 0 for masked logits.
+
+    ``lse`` and (with ``grad_entropy``) ``entropy`` are the forward call's, for
+    the same logits and temperature; incoming gradients have their outputs'
+    dims (any strides), and one that is None counts as zero."""
+    out = _empty(tuple(logits.shape), logits.dtype, logits.device)
+    token_log_probs_backward_into(logits, tokens, out, lse=lse, entropy=entropy, grad_log_probs=grad_log_probs,
+                                  grad_entropy=grad_entropy, grad_lse=grad_lse, temperature=temperature)
+    return out
+
+
+def token_log_probs_backward_into(logits, tokens, out, *, lse, entropy=None, grad_log_probs=None, grad_entropy=None,
+                                  grad_lse=None, temperature: float = 1.0) -> None:
+    """``token_log_probs_backward`` written into an existing C-contiguous tensor."""
+    import torch
+    op = "token_log_probs_backward"
+    fn = _fn("kx_token_log_probs_backward", logits.dtype)
+    h = _bind(logits)
+    same = dict(lse=lse, entropy=entropy, grad_log_probs=grad_log_probs, grad_entropy=grad_entropy,
+                grad_lse=grad_lse, out=out)
+    _same_device(op, h.device, tokens=tokens, **same)
+    _same_dtype(op, logits.dtype, **same)
+    _same_dtype(op, torch.int64, tokens=tokens)
+    err = KxError()
+    raise_for(fn(h.ptr, _ref(logits), _ref(tokens), _ref(lse), _ref(entropy), _ref(grad_log_probs),
+                 _ref(grad_entropy), _ref(grad_lse), float(temperature), _ref(out), C.byref(err)), err)
+
+
+def _lists(op: str, grads, outs=None):
+    """The descriptors of a list of gradients (and of their outputs).  A pair of
+    C-contiguous tensors is described by its elements alone, all such pairs at
+    once: a long list's cost is in this loop."""
+    import torch
+    grads = list(grads)
+    lists = [grads] if outs is None else [grads, list(outs)]
+    if not grads:
+        raise InvalidParameter(f"{op}: grads (at least one)", operation=op, parameter="grads")
+    dtype, dev = grads[0].dtype, _device_index(grads[0])
+    flat = None
+    for name, ts in zip(("grads", "outs"), lists):
+        if len(ts) != len(grads):
+            raise InvalidParameter(f"{op}: {len(ts)} outs for {len(grads)} grads", operation=op, parameter="outs")
+        if any(t.dtype != dtype for t in ts):
+            raise InvalidParameter(f"{op}: {name} of several dtypes", operation=op, parameter=name)
+        if any(_device_index(t) != dev for t in ts):
+            raise InvalidParameter(f"{op}: {name} on several devices", operation=op, parameter=name)
+        here = [isinstance(t, torch.Tensor) and t.is_contiguous() for t in ts]
+        flat = here if flat is None else [a and b for a, b in zip(flat, here)]
+    if outs is not None and any(tuple(g.shape) != tuple(o.shape) for g, o in zip(*lists)):
+        raise LayoutError(f"{op}: output shape mismatch", kind="OutputShapeMismatch")
+    return dtype, [_descriptors(ts, flat) for ts in lists]
+
+
+def _descriptors(ts, flat):
+    arr = (KxTensor * len(ts))()
+    words = np.frombuffer(arr, dtype=np.int64).reshape(len(ts), -1)
+    counts = [t.numel() if f else 0 for t, f in zip(ts, flat)]
+    words[:, 0] = [t.data_ptr() if f else 0 for t, f in zip(ts, flat)]
+    words[:, 1] = words[:, 4] = counts      # storage_len, dims[0]
+    words[:, 3] = 1                         # rank
+    words[:, 4 + MAX_RANK] = 1              # strides[0]
+    for i, f in enumerate(flat):
+        if not f:
+            arr[i] = _descriptor(ts[i])
+    return arr
+
+
+def _norm_call(op: str, grads, outs, max_norm, norm):
+    import torch
+    dtype, arrays = _lists(op, grads, outs)
+    fn = _fn("kx_" + op, dtype)
+    h = _bind(grads[0])
+    if norm is None:
+        norm = torch.empty((), dtype=dtype, device=grads[0].device)
+    _same_device(op, h.device, norm=norm)
+    _same_dtype(op, dtype, norm=norm)
+    n = len(arrays[0])
+    size = C.c_uint64()
+    raise_for(lib.kx_grad_norm_workspace(n, C.byref(size)), None)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=grads[0].device)
+    err = KxError()
+    tail = (_ref(norm), ws.data_ptr(), size.value, C.byref(err))
+    if outs is None:
+        rc = fn(h.ptr, arrays[0], n, *tail)
+    else:
+        rc = fn(h.ptr, arrays[0], n, float(max_norm), arrays[1], *tail)
+    raise_for(rc, err)
+    return norm
+
+
+def grad_norm(grads):
+    """The 2-norm over all elements of a list of gradients of one dtype (any
+    shapes and strides), as a tensor without axes.  Does not wait for the
+    device."""
+    return _norm_call("grad_norm", list(grads), None, None, None)
+
+
+def grad_norm_into(grads, out) -> None:
+    """``grad_norm`` written into an existing tensor of one element."""
+    _norm_call("grad_norm", list(grads), None, None, out)
+
+
+def clip_grad_norm(grads, max_norm: float):
+    """(norm, clipped): the global 2-norm of ``grads`` and new tensors that hold
+    them scaled by ``min(1, max_norm / norm)``.  Where the norm is at most
+    ``max_norm``, or is not finite, they are the gradients as they were."""
+    import torch
+    grads = list(grads)
+    outs = [torch.empty_like(g) if isinstance(g, torch.Tensor) else _empty(tuple(g.shape), g.dtype, g.device)
+            for g in grads]
+    return clip_grad_norm_into(grads, max_norm, outs), outs
+
+
+def clip_grad_norm_into(grads, max_norm: float, outs, norm=None):
+    """``clip_grad_norm`` written into existing tensors, and the norm, into
+    ``norm`` if one is given.  Each output may be its gradient itself: pass
+    ``grads`` twice to clip in place."""
+    return _norm_call("clip_grad_norm", list(grads), list(outs), max_norm, norm)
 
 
 # ---------------------------------------------------------------------------
