@@ -10,12 +10,17 @@
 // A logit of -inf is a token that a mask took out: probability 0, no part in
 // the entropy, gradient 0.  Nothing here is read back by the host: rows that
 // hold a NaN or +inf answer with NaN.
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <cstring>
 
 #include "kx_internal.hpp"
 
+namespace cg = cooperative_groups;
 using namespace kx;
 
 namespace {
@@ -42,141 +47,403 @@ __device__ __forceinline__ int64_t row_offset(const Rows &g, int which, int64_t 
     return g.ndims > 0 ? o + row * g.str[which][0] : o;
 }
 
-template <typename T> __device__ __forceinline__ T kexp(T x);
-template <> __device__ __forceinline__ float kexp<float>(float x) { return expf(x); }
-template <> __device__ __forceinline__ double kexp<double>(double x) { return exp(x); }
-
-// The smallest (x - m)/T that enters a sum: exp of it is 0 in either type, and
-// 0 times it is 0 where 0 times -inf would be NaN.
-template <typename T> __device__ __forceinline__ T floor_of(T d) { return fmax(d, T(-1e5)); }
-
 template <typename T> struct ForwardParams {
     const T *x;
     const int64_t *tokens;
     T *log_probs, *lse, *entropy, *top_lp;
     int64_t *top_ids;
-    int64_t len, stride;
-    int top;
-    T temperature;
+    int64_t stride;
+    int len, top, cluster;   // cluster: blocks that share a row
+    T temperature, factor;   // factor: exp_factor(temperature)
     Rows rows;
 };
 
-template <typename T>
-__device__ __forceinline__ T block_sum(T v, T *red) {
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    using type = float4;
+    static constexpr int n = 4;
+};
+template <> struct Vec<double> {
+    using type = double2;
+    static constexpr int n = 2;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp((x - m)/T) of a difference d = x - m <= 0.  f32: 2^(d c), c = log2(e)/T,
+// by the special-function unit, whose few half steps of error are below those
+// of the difference itself; results under the smallest normal number are 0.
+__device__ __forceinline__ float exp_scaled(float d, float c) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * c));
+    return e;
+}
+__device__ __forceinline__ double exp_scaled(double d, double c) { return exp(d * c); }
+template <typename T> T exp_factor(T temperature);
+template <> float exp_factor<float>(float t) { return kLog2e / t; }
+template <> double exp_factor<double>(double t) { return 1.0 / t; }
+
+template <typename T> __device__ __forceinline__ T lowest();
+template <> __device__ __forceinline__ float lowest<float>() { return -FLT_MAX; }
+template <> __device__ __forceinline__ double lowest<double>() { return -DBL_MAX; }
+// A difference before it is multiplied by its exponential, which is 0 if the
+// difference is -inf: their product has to be 0, not NaN.
+template <typename T> __device__ __forceinline__ T finite(T d) { return fmax(d, lowest<T>()); }
+
+// What a thread knows of the elements that it has seen: their maximum, the sum
+// of exp((x - m)/T) and that of exp((x - m)/T) (x - m).  A NaN or +inf makes
+// the sum NaN; it stays 0 where all elements are -inf, which makes -inf the
+// neutral element that fills up a last vector.
+template <typename T, bool ENT> struct Stats {
+    T m = lowest<T>(), s = T(0), e = T(0);
+
+    template <int N> __device__ __forceinline__ void add(const T (&v)[N], T c) {
+        T nm = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    T s = T(0);
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) s += red[w];
-    return s;
-}
-
-template <typename T>
-__device__ __forceinline__ T block_max(T v, T *red) {
+        for (int i = 0; i < N; ++i) nm = fmax(nm, v[i]);
+        // an f64 exponential costs far more than the branch around it
+        if (sizeof(T) == 4 || nm != m) rebase(nm, c);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    T s = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) s = fmax(s, red[w]);
-    return s;
-}
-
-// Maximum, sum of exponentials and sum of exponential times difference of one
-// row, by all threads of the block.
-template <typename T>
-__device__ void row_stats(const T *x, int64_t len, int64_t stride, T temperature, T *red, T &m, T &s, T &e) {
-    m = -INFINITY;
-    for (int64_t j = threadIdx.x; j < len; j += blockDim.x) m = fmax(m, x[j * stride]);
-    m = block_max(m, red);
-    const T base = m == T(-INFINITY) ? T(0) : m;
-    s = T(0);
-    e = T(0);
-    for (int64_t j = threadIdx.x; j < len; j += blockDim.x) {
-        const T d = (x[j * stride] - base) / temperature;
-        const T p = kexp(d);
-        s += p;
-        e += p * floor_of(d);
-    }
-    s = block_sum(s, red);
-    e = block_sum(e, red);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
-    __shared__ T red[8];
-    __shared__ T best_v[8];
-    __shared__ int64_t best_i[8];
-    for (int64_t row = blockIdx.x; row < p.rows.count; row += gridDim.x) {
-        const T *x = p.x + row_offset(p.rows, kLogits, row);
-        T m, s, e;
-        row_stats(x, p.len, p.stride, p.temperature, red, m, s, e);
-        const bool bad = isnan(s), none = !bad && m == T(-INFINITY);
-        const double log_s = log((double)s);
-        if (threadIdx.x == 0) {
-            if (p.lse) p.lse[row] = bad ? T(NAN) : none ? T(-INFINITY) : (T)((double)m / (double)p.temperature + log_s);
-            if (p.entropy) p.entropy[row] = bad ? T(NAN) : none ? T(0) : (T)(log_s - (double)e / (double)s);
-            if (p.log_probs) {
-                const int64_t t = p.tokens[row_offset(p.rows, kTokens, row)];
-                T lp = T(0);
-                if (t >= p.len) lp = T(NAN);
-                else if (t >= 0)
-                    lp = bad ? T(NAN) : none ? T(-INFINITY)
-                             : (T)(((double)x[t * p.stride] - (double)m) / (double)p.temperature - log_s);
-                p.log_probs[row] = lp;
-            }
+        for (int i = 0; i < N; ++i) {
+            const T d = v[i] - m, p = exp_scaled(d, c);
+            s += p;
+            if (ENT) e = fma(p, finite(d), e);
         }
-        // the alternatives, one pass each: the best element after the last one
-        T last_v = INFINITY;
-        int64_t last_i = -1;
-        for (int k = 0; k < p.top; ++k) {
-            T v = -INFINITY;
-            int64_t i = INT64_MAX;
-            if (!bad) {
-                for (int64_t j = threadIdx.x; j < p.len; j += blockDim.x) {
-                    const T c = x[j * p.stride];
-                    if ((c < last_v || (c == last_v && j > last_i)) && (c > v || (c == v && j < i))) {
-                        v = c;
-                        i = j;
+    }
+    __device__ __forceinline__ void rebase(T nm, T c) {
+        const T d = m - nm, f = exp_scaled(d, c);
+        if (ENT) e = f == T(0) ? T(0) : fma(d, s, e) * f;
+        s *= f;
+        m = nm;
+    }
+    // over the warp's lanes, the same in each
+    __device__ __forceinline__ void join(T c) {
+        T nm = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) nm = fmax(nm, __shfl_xor_sync(0xffffffffu, nm, o));
+        rebase(nm, c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (ENT) e += __shfl_xor_sync(0xffffffffu, e, o);
+        }
+    }
+};
+
+// One row's elements as this block walks them: a head up to the first 16-byte
+// boundary, vectors, a tail; or single elements of any stride.
+template <typename T, bool VEC> struct RowView {
+    static constexpr int VN = VEC ? Vec<T>::n : 1;
+    const T *x;
+    int64_t stride;
+    int head, tail, nv;   // elements before the vectors, after them; vectors
+
+    __device__ __forceinline__ RowView(const T *row, int len, int64_t stride_) : x(row), stride(stride_) {
+        if (VEC) {
+            const int to = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+            head = to < len ? to : len;
+            nv = (len - head) / VN;
+            tail = len - head - nv * VN;
+        } else {
+            head = tail = 0;
+            nv = len;
+        }
+    }
+    __device__ __forceinline__ void load(int i, bool ok, T (&v)[VN]) const {
+        if (VEC) {
+            typename Vec<T>::type q;
+            if (ok) q = __ldg(reinterpret_cast<const typename Vec<T>::type *>(x + head) + i);
+#pragma unroll
+            for (int k = 0; k < VN; ++k) v[k] = ok ? reinterpret_cast<const T *>(&q)[k] : T(-INFINITY);
+        } else {
+            v[0] = ok ? __ldg(x + i * stride) : T(-INFINITY);
+        }
+    }
+    __device__ __forceinline__ T at(int j) const { return __ldg(x + j * stride); }
+};
+
+// a before b in the order of the alternatives
+template <typename T> __device__ __forceinline__ bool before(T av, int ai, T bv, int bi) {
+    return av > bv || (av == bv && ai < bi);
+}
+
+// The warp's lane values in falling order over its lanes (a bitonic network).
+template <typename T> __device__ __forceinline__ T sorted_falling(T v, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const T o = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool up = (lane & j) == 0, falling = (lane & k) == 0;
+            v = up == falling ? fmax(v, o) : fmin(v, o);
+        }
+    }
+    return v;
+}
+
+constexpr int kCandidates = 512;
+
+template <typename T, int NW> struct Shared {
+    T m[NW], s[NW], e[NW], bound[NW];     // each warp's
+    T cta_m, cta_s, cta_e;                // the block's, for its cluster
+    int found;
+    T best_v[32];                         // the block's alternatives, in order
+    int best_i[32];
+    T cand_v[kCandidates];
+    int cand_i[kCandidates];
+};
+
+// The forward pass.  One pass over the logits keeps, for each thread, the
+// maximum of its elements and the two sums against it; they meet by shuffles,
+// then in shared memory, then (few rows) over the cluster's shared memory, so
+// that one launch and no workspace do for any number of rows.  The bound is
+// the reading of the logits; the instructions for an element are about eight.
+//
+// The alternatives come from the threads' maxima: the K-th largest of them, or
+// less, bounds the K-th alternative from below, so only elements at or above
+// it matter, and only the threads whose maximum reaches it read theirs again
+// (about K of them, from the cache).  A few dozen candidates are ranked by
+// counting.  Should more than kCandidates elements reach the bound (rows of
+// equal values), the alternatives are found one after another instead.
+template <typename T, bool VEC, bool ENT, int NW>
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
+    constexpr int kRowsPerBlock = NW == 1 ? 4 : 1;
+    constexpr int GT = NW * 32;           // threads that share a row in this block
+    constexpr int VN = RowView<T, VEC>::VN;
+    constexpr int U = VEC ? 4 : 8;        // loads in flight for each thread
+    __shared__ Shared<T, NW> shared[kRowsPerBlock];
+    const int lane = threadIdx.x & 31;
+    const int warp = NW == 1 ? 0 : threadIdx.x >> 5;
+    const int tid = NW == 1 ? lane : threadIdx.x;
+    Shared<T, NW> &sh = shared[NW == 1 ? threadIdx.x >> 5 : 0];
+    auto sync = [] {
+        if (NW == 1) __syncwarp();
+        else __syncthreads();
+    };
+    const int C = NW == 1 ? 1 : p.cluster;
+    const int rank = NW == 1 ? 0 : blockIdx.x % C;
+    const T c = p.factor;
+    const int64_t step = (int64_t)(gridDim.x / C) * kRowsPerBlock;
+    for (int64_t row = (int64_t)(blockIdx.x / C) * kRowsPerBlock + (NW == 1 ? threadIdx.x >> 5 : 0);
+         row < p.rows.count; row += step) {
+        const RowView<T, VEC> x(p.x + row_offset(p.rows, kLogits, row), p.len, p.stride);
+        // the given token's logit, on its way while the row is read
+        int64_t token = -1;
+        T given = T(NAN);
+        if (p.log_probs && rank == 0 && tid == 0) {
+            token = p.tokens[row_offset(p.rows, kTokens, row)];
+            if (token >= 0 && token < p.len) given = x.at((int)token);
+        }
+        const int per = (x.nv + C - 1) / C;
+        const int v0 = min(rank * per, x.nv), v1 = min(v0 + per, x.nv);
+        const bool edges = VEC && rank == 0 && warp == 0;   // the warp of the head and the tail
+        const int tail0 = x.head + x.nv * VN;
+        Stats<T, ENT> st;
+        if (edges) {
+            const T v[1] = {lane < x.head ? x.at(lane) : T(-INFINITY)};
+            st.add(v, c);
+        }
+        for (int i = v0 + tid; i < v1; i += GT * U) {
+            T v[U][VN];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
+            st.add(reinterpret_cast<T(&)[U * VN]>(v), c);
+        }
+        if (edges) {
+            const T v[1] = {lane < x.tail ? x.at(tail0 + lane) : T(-INFINITY)};
+            st.add(v, c);
+        }
+        const T mine = st.m;
+        st.join(c);
+        T bound = lowest<T>();
+        if (p.top > 0) {
+            // NW times the (K / NW)-th largest maximum of a warp are K elements
+            const T sorted = sorted_falling(mine, lane);
+            bound = __shfl_sync(0xffffffffu, sorted, (p.top + NW - 1) / NW - 1);
+        }
+        if (NW > 1) {
+            if (lane == 0) {
+                sh.m[warp] = st.m;
+                sh.s[warp] = st.s;
+                sh.e[warp] = st.e;
+                sh.bound[warp] = bound;
+            }
+            if (tid == 0) sh.found = 0;
+            sync();
+            st.m = lane < NW ? sh.m[lane % NW] : lowest<T>();
+            st.s = lane < NW ? sh.s[lane % NW] : T(0);
+            st.e = lane < NW ? sh.e[lane % NW] : T(0);
+            st.join(c);
+            if (p.top > 0) {
+#pragma unroll
+                for (int w = 0; w < NW; ++w) bound = fmin(bound, sh.bound[w]);
+            }
+        } else {
+            if (tid == 0) sh.found = 0;
+            sync();
+        }
+        if (p.top > 0) {
+            auto offer = [&](T v, int j) {
+                if (v >= bound && v > T(-INFINITY)) {
+                    const int k = atomicAdd(&sh.found, 1);
+                    if (k < kCandidates) {
+                        sh.cand_v[k] = v;
+                        sh.cand_i[k] = j;
+                    }
+                }
+            };
+            if (mine >= bound) {
+                for (int i = v0 + tid; i < v1; i += GT * U) {
+                    T v[U][VN];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int k = 0; k < VN; ++k) offer(v[u][k], x.head + (i + u * GT) * VN + k);
+                }
+                if (edges && lane < x.head) offer(x.at(lane), lane);
+                if (edges && lane < x.tail) offer(x.at(tail0 + lane), tail0 + lane);
+            }
+            sync();
+            const int n = sh.found;
+            if (n <= kCandidates) {
+                for (int k = tid; k < p.top; k += GT) {
+                    if (k >= n) {
+                        sh.best_v[k] = T(-INFINITY);
+                        sh.best_i[k] = INT_MAX;
+                    }
+                }
+                for (int k = tid; k < n; k += GT) {
+                    const T v = sh.cand_v[k];
+                    const int j = sh.cand_i[k];
+                    int r = 0;
+                    for (int o = 0; o < n; ++o) r += before(sh.cand_v[o], sh.cand_i[o], v, j);
+                    if (r < p.top) {
+                        sh.best_v[r] = v;
+                        sh.best_i[r] = j;
+                    }
+                }
+            } else {
+                T last_v = T(INFINITY);
+                int last_i = -1;
+                for (int k = 0; k < p.top; ++k) {
+                    T bv = T(-INFINITY);
+                    int bi = INT_MAX;
+                    auto look = [&](T v, int j) {
+                        if (before(last_v, last_i, v, j) && before(v, j, bv, bi)) {
+                            bv = v;
+                            bi = j;
+                        }
+                    };
+                    for (int i = v0 + tid; i < v1; i += GT) {
+                        T v[VN];
+                        x.load(i, true, v);
+#pragma unroll
+                        for (int q = 0; q < VN; ++q) look(v[q], x.head + i * VN + q);
+                    }
+                    if (edges && lane < x.head) look(x.at(lane), lane);
+                    if (edges && lane < x.tail) look(x.at(tail0 + lane), tail0 + lane);
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const T ov = __shfl_xor_sync(0xffffffffu, bv, o);
+                        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+                        if (before(ov, oi, bv, bi)) {
+                            bv = ov;
+                            bi = oi;
+                        }
+                    }
+                    if (NW > 1) {
+                        sync();
+                        if (lane == 0) {
+                            sh.cand_v[warp] = bv;
+                            sh.cand_i[warp] = bi;
+                        }
+                        sync();
+#pragma unroll
+                        for (int w = 0; w < NW; ++w)
+                            if (before(sh.cand_v[w], sh.cand_i[w], bv, bi)) {
+                                bv = sh.cand_v[w];
+                                bi = sh.cand_i[w];
+                            }
+                    }
+                    if (tid == 0) {
+                        sh.best_v[k] = bv;
+                        sh.best_i[k] = bi;
+                    }
+                    last_v = bv;
+                    last_i = bi;
+                }
+            }
+            sync();
+        }
+        int total = p.top;      // alternatives in best_*, in order
+        if (NW > 1 && C > 1) {
+            cg::cluster_group cluster = cg::this_cluster();
+            if (tid == 0) {
+                sh.cta_m = st.m;
+                sh.cta_s = st.s;
+                sh.cta_e = st.e;
+            }
+            cluster.sync();
+            if (rank == 0) {
+                const Shared<T, NW> *other = cluster.map_shared_rank(&sh, lane < C ? lane : 0);
+                st.m = lane < C ? other->cta_m : lowest<T>();
+                st.s = lane < C ? other->cta_s : T(0);
+                st.e = lane < C ? other->cta_e : T(0);
+                st.join(c);
+                if (p.top > 0) {
+                    total = C * p.top;
+                    for (int k = tid; k < total; k += GT) {
+                        const Shared<T, NW> *from = cluster.map_shared_rank(&sh, k / p.top);
+                        sh.cand_v[k] = from->best_v[k % p.top];
+                        sh.cand_i[k] = from->best_i[k % p.top];
                     }
                 }
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const T ov = __shfl_xor_sync(0xffffffffu, v, o);
-                const int64_t oi = __shfl_xor_sync(0xffffffffu, i, o);
-                if (ov > v || (ov == v && oi < i)) {
-                    v = ov;
-                    i = oi;
-                }
-            }
-            __syncthreads();
-            if ((threadIdx.x & 31) == 0) {
-                best_v[threadIdx.x >> 5] = v;
-                best_i[threadIdx.x >> 5] = i;
-            }
-            __syncthreads();
-            v = best_v[0];
-            i = best_i[0];
-            for (int w = 1; w < 8; ++w)
-                if (best_v[w] > v || (best_v[w] == v && best_i[w] < i)) {
-                    v = best_v[w];
-                    i = best_i[w];
-                }
-            if (threadIdx.x == 0) {
-                const bool gone = v == T(-INFINITY);
-                p.top_lp[row * p.top + k] =
-                    bad ? T(NAN) : gone ? T(-INFINITY)
-                                        : (T)(((double)v - (double)m) / (double)p.temperature - log_s);
-                p.top_ids[row * p.top + k] = bad || gone ? -1 : i;
-            }
-            last_v = v;
-            last_i = i;
+            cluster.sync();     // the others' shared memory is read
+            if (rank != 0) continue;
         }
-        __syncthreads();
+        // the row's answers, in 64 bits up to their rounding
+        const bool bad = isnan(st.s), none = st.s == T(0);
+        const double temperature = (double)p.temperature, m = (double)st.m;
+        const double log_s = none ? 0.0 : log((double)st.s);
+        auto log_prob = [&](T v) {
+            if (bad) return T(NAN);
+            if (v == T(-INFINITY)) return T(-INFINITY);
+            return (T)(((double)v - m) / temperature - log_s);
+        };
+        if (tid == 0) {
+            if (p.lse) p.lse[row] = bad ? T(NAN) : none ? T(-INFINITY) : (T)(m / temperature + log_s);
+            if (ENT && p.entropy) {
+                const double mean = none ? 0.0 : (double)st.e / (double)st.s / temperature;
+                p.entropy[row] = bad ? T(NAN) : (T)(log_s - mean);
+            }
+            if (p.log_probs) p.log_probs[row] = token < 0 ? T(0) : token >= p.len ? T(NAN) : log_prob(given);
+        }
+        if (p.top > 0) {
+            for (int k = tid; k < total; k += GT) {
+                T v = sh.best_v[k % p.top];
+                int j = sh.best_i[k % p.top], r = k;
+                if (total > p.top) {
+                    // lists of the cluster's blocks: each in order, so the
+                    // place in them all is counted; what a list lacks stands
+                    // behind all that is there, in the order of the lists
+                    v = sh.cand_v[k];
+                    j = sh.cand_i[k];
+                    r = 0;
+                    for (int o = 0; o < total; ++o) {
+                        const T ov = sh.cand_v[o];
+                        const int oj = sh.cand_i[o];
+                        r += before(ov, oj, v, j) || (ov == v && oj == j && o < k);
+                    }
+                    if (r >= p.top) continue;
+                }
+                p.top_lp[row * p.top + r] = log_prob(v);
+                p.top_ids[row * p.top + r] = bad || v == T(-INFINITY) ? -1 : j;
+            }
+        }
+        sync();     // the next row's candidates overwrite these
     }
 }
 
@@ -184,8 +451,9 @@ template <typename T> struct BackwardParams {
     const T *x, *lse, *entropy, *g_lp, *g_h, *g_lse;
     const int64_t *tokens;
     T *out;
-    int64_t len, stride;
-    T temperature;
+    int64_t stride;
+    int len, per, parts;     // elements of one block's part of a row; parts of a row
+    T temperature, factor;
     Rows rows;
 };
 
@@ -194,41 +462,130 @@ template <typename T> struct BackwardParams {
 // anew instead.
 constexpr double kLseTrusted = 256.0;
 
-template <typename T>
-__global__ void __launch_bounds__(256) log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
-    __shared__ T red[8];
-    for (int64_t row = blockIdx.x; row < p.rows.count; row += gridDim.x) {
-        const T *x = p.x + row_offset(p.rows, kLogits, row);
+// log p as the exponential below takes it: in units of log 2 for f32.
+constexpr double kUnit32 = 1.4426950408889634;
+template <typename T> __device__ __forceinline__ double log_unit() { return sizeof(T) == 4 ? kUnit32 : 1.0; }
+__device__ __forceinline__ float exp_unit(float a) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a));
+    return e;
+}
+__device__ __forceinline__ double exp_unit(double a) { return exp(a); }
+
+// A row's numbers in the gradient of its elements:
+//   log p = (x - base) c - less,  dx = p (a - b log p)  [+ at the token]
+template <typename T> struct RowGrad {
+    T base, less, a, b, at_token;
+    int token;
+    __device__ __forceinline__ T operator()(T v, T c) const {
+        const T lq = fma(v - base, c, -less);
+        const T d = exp_unit(lq) * fma(-b, fmax(lq, T(-1e5)), a);
+        return v == T(-INFINITY) ? T(0) : d;
+    }
+};
+
+// Elements lo to hi of the row whose logits x walks and whose gradient is out.
+template <typename T, bool VEC, int THREADS>
+__device__ __forceinline__ void grad_part(const RowView<T, VEC> &x, T *out, int lo, int hi, const RowGrad<T> &g, T c,
+                                          bool first, bool last) {
+    constexpr int VN = RowView<T, VEC>::VN;
+    constexpr int U = VEC ? 4 : 8;
+    auto one = [&](int j) {
+        const T v = x.at(j);
+        T d = g(v, c);
+        if (j == g.token && v != T(-INFINITY)) d += g.at_token;
+        out[j] = d;
+    };
+    for (int i = lo + (int)threadIdx.x; i < hi; i += THREADS * U) {
+        T v[U][VN];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x.load(i + u * THREADS, i + u * THREADS < hi, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = x.head + (i + u * THREADS) * VN;
+            T d[VN];
+#pragma unroll
+            for (int k = 0; k < VN; ++k) d[k] = g(v[u][k], c);
+            if ((unsigned)(g.token - j) < (unsigned)VN) {
+#pragma unroll
+                for (int k = 0; k < VN; ++k)
+                    if (g.token == j + k && v[u][k] != T(-INFINITY)) d[k] += g.at_token;
+            }
+            if (i + u * THREADS < hi) {
+                if (VEC) *reinterpret_cast<typename Vec<T>::type *>(out + j) = *reinterpret_cast<const typename Vec<T>::type *>(d);
+                else out[j] = d[0];
+            }
+        }
+    }
+    if (VEC && first && (int)threadIdx.x < x.head) one(threadIdx.x);
+    if (VEC && last && (int)threadIdx.x < x.tail) one(x.head + x.nv * VN + threadIdx.x);
+}
+
+constexpr int kGradThreads = 256;
+
+// The gradient: one element in, one out, with a row's few numbers between
+// them.  The bound is the two streams; a block takes a part of one row.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
+    constexpr int NW = kGradThreads / 32;
+    __shared__ T sm[NW], ss[NW];
+    const T c = p.factor;
+    const int64_t total = p.rows.count * p.parts;
+    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+        const int64_t row = w / p.parts;
+        const int part = (int)(w - row * p.parts);
+        const T *xr = p.x + row_offset(p.rows, kLogits, row);
         T *out = p.out + row * p.len;
         const double lse = (double)p.lse[row_offset(p.rows, kLse, row)];
-        T base, less;   // log p = (x - base)/T - less
+        const double temperature = (double)p.temperature, unit = log_unit<T>();
+        RowGrad<T> g;
         if (fabs(lse) <= kLseTrusted) {
-            const double b = lse * (double)p.temperature;
-            base = (T)b;
-            less = (T)((b - (double)base) / (double)p.temperature);
+            const double b = lse * temperature;
+            g.base = (T)b;
+            g.less = (T)((b - (double)g.base) / temperature * unit);
         } else {
-            T m, s, e;
-            row_stats(x, p.len, p.stride, p.temperature, red, m, s, e);
-            base = m;
-            less = isnan(s) ? T(NAN) : (T)log((double)s);
+            const RowView<T, VEC> x(xr, p.len, p.stride);
+            Stats<T, false> st;
+            for (int j = threadIdx.x; j < p.len; j += kGradThreads) {
+                const T v[1] = {x.at(j)};
+                st.add(v, c);
+            }
+            st.join(c);
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) {
+                sm[threadIdx.x >> 5] = st.m;
+                ss[threadIdx.x >> 5] = st.s;
+            }
+            __syncthreads();
+            const int k = threadIdx.x & 31;
+            st.m = k < NW ? sm[k % NW] : lowest<T>();
+            st.s = k < NW ? ss[k % NW] : T(0);
+            st.join(c);
+            g.base = st.m;
+            g.less = (T)(log((double)st.s) * unit);
         }
         const int64_t t = p.tokens ? p.tokens[row_offset(p.rows, kTokens, row)] : -1;
-        T g = p.g_lp && t >= 0 ? p.g_lp[row_offset(p.rows, kGradLp, row)] : T(0);
+        T gp = p.g_lp && t >= 0 ? p.g_lp[row_offset(p.rows, kGradLp, row)] : T(0);
+        if (t >= p.len) gp = T(NAN);
         const T gh = p.g_h ? p.g_h[row_offset(p.rows, kGradH, row)] : T(0);
         const T h = p.g_h ? p.entropy[row_offset(p.rows, kEntropy, row)] : T(0);
         const T gl = p.g_lse ? p.g_lse[row_offset(p.rows, kGradLse, row)] : T(0);
-        if (p.g_lp && t >= p.len) g = T(NAN);
-        const T factor = (gl - g - gh * h) / p.temperature;
-        const T gh_t = gh / p.temperature, g_t = g / p.temperature;
-        for (int64_t j = threadIdx.x; j < p.len; j += blockDim.x) {
-            const T v = x[j * p.stride];
-            const T lq = (v - base) / p.temperature - less;
-            const T q = kexp(lq);
-            T d = q * (factor - gh_t * floor_of(lq));
-            if (j == t) d += g_t;
-            out[j] = v == T(-INFINITY) ? T(0) : d;
+        g.a = (gl - gp - gh * h) / p.temperature;
+        g.b = (T)((double)gh / temperature / unit);
+        g.at_token = gp / p.temperature;
+        g.token = t >= 0 && t < p.len ? (int)t : -1;
+        // vectors where logits and gradient lie alike against 16 bytes
+        const bool alike = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+        if (VEC && alike) {
+            const RowView<T, true> x(xr, p.len, p.stride);
+            const int per = p.per / RowView<T, true>::VN;
+            const int lo = min(part * per, x.nv), hi = part + 1 == p.parts ? x.nv : min(lo + per, x.nv);
+            grad_part<T, true, kGradThreads>(x, out, lo, hi, g, c, part == 0, part + 1 == p.parts);
+        } else {
+            const RowView<T, false> x(xr, p.len, p.stride);
+            const int lo = min(part * p.per, p.len), hi = part + 1 == p.parts ? p.len : min(lo + p.per, p.len);
+            grad_part<T, false, kGradThreads>(x, out, lo, hi, g, c, false, false);
         }
-        __syncthreads();
     }
 }
 
@@ -238,9 +595,14 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(const __grid_co
 const char *const kFwd = "token_log_probs";
 const char *const kBwd = "token_log_probs_backward";
 
+constexpr int64_t kMaxGrid = 1 << 30;
+constexpr int kRowWarps = 8;
+constexpr int kGradPart = 8192;   // elements of a block's part of a row in the gradient
+constexpr int kWarpRow = 2048;    // longest row that one warp takes
+
 // The temperature divides logits: it and its reciprocal are normal numbers.
 template <typename T> bool temperature_ok(T t) {
-    return std::isnormal((double)t) && t > T(0) && std::isnormal((T)(T(1.4426950408889634) / t));
+    return std::isnormal((double)t) && t > T(0) && std::isnormal(exp_factor<T>(t));
 }
 
 // An operand with one element for each row: the logits' dims without the last.
@@ -322,8 +684,8 @@ int check_logits(const kx_tensor *logits, T temperature, const char *op, Span *s
     int rc = validate_tensor(logits, sizeof(T), s, err);
     if (rc) return rc;
     if (logits->rank == 0) return set_err(err, KX_E_INVALID_RANK, op, "rank", 1, 0);
-    if (logits->dims[logits->rank - 1] > (uint64_t)INT32_MAX)
-        return set_err(err, KX_E_UNSUPPORTED, op, "vocabulary above 2^31-1");
+    if (logits->dims[logits->rank - 1] > (1u << 30))
+        return set_err(err, KX_E_UNSUPPORTED, op, "vocabulary above 2^30");
     // with an empty vocabulary the rows alone need not fit the element count
     rc = validate_dims(logits->dims, logits->rank - 1, err);
     if (rc) return rc;
@@ -344,6 +706,31 @@ int row_output(const kx_tensor *t, const kx_tensor *logits, uint32_t es, const c
     if (!is_c_contiguous(t))
         return set_err(err, KX_E_LAYOUT, op, "output must be C-contiguous", KX_LAYOUT_OUTPUT_NOT_C_CONTIGUOUS);
     return seen->add(t, s, es, true, op, err);
+}
+
+template <typename T, bool VEC, bool ENT>
+void launch_forward(Handle *h, ForwardParams<T> &p) {
+    if (p.len <= kWarpRow) {
+        const int64_t blocks = (p.rows.count + 3) / 4;
+        log_probs_kernel<T, VEC, ENT, 1><<<(unsigned)std::min<int64_t>(blocks, kMaxGrid), 128, 0, h->stream>>>(p);
+        h->last_kernel = "log_probs_warp";
+        return;
+    }
+    while (p.cluster < 8 && p.rows.count * p.cluster < 2 * h->sm_count && p.len / (2 * p.cluster) >= 4096)
+        p.cluster *= 2;
+    const int64_t rows = std::min<int64_t>(p.rows.count, kMaxGrid / p.cluster);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * p.cluster));
+    cfg.blockDim = dim3(kRowWarps * 32);
+    cfg.stream = h->stream;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)p.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, log_probs_kernel<T, VEC, ENT, kRowWarps>, p);
+    h->last_kernel = p.cluster > 1 ? "log_probs_cluster" : "log_probs_block";
 }
 
 template <typename T>
@@ -407,22 +794,23 @@ int forward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *tokens
     p.entropy = at<T>(entropy);
     p.top_lp = at<T>(top_log_probs);
     p.top_ids = at<int64_t>(top_tokens);
-    p.len = (int64_t)logits->dims[logits->rank - 1];
+    p.len = (int)logits->dims[logits->rank - 1];
     p.stride = logits->strides[logits->rank - 1];
     p.top = (int)top;
     p.temperature = temperature;
+    p.factor = exp_factor<T>(temperature);
+    p.cluster = 1;
     DeviceGuard guard(h->device);
     if (!guard.ok) return set_err(err, KX_E_NO_DEVICE, kFwd, "cannot select device");
-    const int64_t cap = 16LL * h->sm_count;
-    const unsigned grid = (unsigned)(p.rows.count < cap ? p.rows.count : cap);
-    log_probs_kernel<T><<<grid, 256, 0, h->stream>>>(p);
+    const bool vec = p.stride == 1 || p.len <= 1;
+    if (vec) entropy ? launch_forward<T, true, true>(h, p) : launch_forward<T, true, false>(h, p);
+    else entropy ? launch_forward<T, false, true>(h, p) : launch_forward<T, false, false>(h, p);
     const cudaError_t ce = cudaGetLastError();
     if (ce != cudaSuccess) {
         h->cuda_fail(ce);
         return cuda_err(err, h, kFwd);
     }
     ++h->launches;
-    h->last_kernel = "log_probs";
     return KX_OK;
 }
 
@@ -487,14 +875,18 @@ int backward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *token
     p.g_h = at<T>(grad_entropy);
     p.g_lse = at<T>(grad_lse);
     p.out = at<T>(grad_logits);
-    p.len = (int64_t)logits->dims[logits->rank - 1];
+    p.len = (int)logits->dims[logits->rank - 1];
     p.stride = logits->strides[logits->rank - 1];
     p.temperature = temperature;
+    p.factor = exp_factor<T>(temperature);
+    p.per = kGradPart;
+    p.parts = std::max(1, (p.len + p.per - 1) / p.per);
     DeviceGuard guard(h->device);
     if (!guard.ok) return set_err(err, KX_E_NO_DEVICE, kBwd, "cannot select device");
-    const int64_t cap = 16LL * h->sm_count;
-    const unsigned grid = (unsigned)(p.rows.count < cap ? p.rows.count : cap);
-    log_probs_backward_kernel<T><<<grid, 256, 0, h->stream>>>(p);
+    const bool vec = p.stride == 1 || p.len <= 1;
+    const unsigned grid = (unsigned)std::min<i128>((i128)p.rows.count * p.parts, kMaxGrid);
+    if (vec) log_probs_backward_kernel<T, true><<<grid, kGradThreads, 0, h->stream>>>(p);
+    else log_probs_backward_kernel<T, false><<<grid, kGradThreads, 0, h->stream>>>(p);
     const cudaError_t ce = cudaGetLastError();
     if (ce != cudaSuccess) {
         h->cuda_fail(ce);
