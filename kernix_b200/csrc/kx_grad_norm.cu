@@ -21,6 +21,45 @@ namespace {
 const char *const kNorm = "grad_norm";
 const char *const kClip = "clip_grad_norm";
 constexpr int kThreads = 256;
+constexpr int kSpans = 256;     // tensors of one launch
+constexpr int kVectors = 4;     // 16-byte loads in flight for each thread
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    using type = float4;
+    static constexpr int n = 4;
+};
+template <> struct Vec<double> {
+    using type = double2;
+    static constexpr int n = 2;
+};
+template <typename T> constexpr int kChunk = kThreads * kVectors * Vec<T>::n;   // elements
+
+// Tensors whose elements fill their span, in whatever order, as runs of
+// memory cut into chunks; a launch's parameters hold the list, so a captured
+// graph keeps it.
+template <typename T> struct Spans {
+    int n;
+    uint32_t chunks;
+    const T *src[kSpans];
+    int64_t len[kSpans];
+    uint32_t first[kSpans + 1];     // each span's first chunk, then their number
+};
+template <typename T> struct Outputs {
+    T *dst[kSpans];
+};
+
+// A span's elements before its first 16-byte boundary, its vectors, the rest.
+template <typename T> struct Cut {
+    int head, tail;
+    int64_t nv;
+    __device__ __forceinline__ Cut(const T *p, int64_t len) {
+        const int to = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T);
+        head = to < len ? to : (int)len;
+        nv = (len - head) / Vec<T>::n;
+        tail = (int)(len - head - nv * Vec<T>::n);
+    }
+};
 
 // One tensor (and its scaled copy) as C-order dims with each one's strides.
 struct Geom {
@@ -39,19 +78,77 @@ __device__ __forceinline__ void offsets(const Geom &g, int64_t i, int64_t &so, i
     }
 }
 
+// The same total in each thread of the block, of which this is the one call.
 __device__ double block_total(double v) {
-    __shared__ double red[kThreads / 32];
+    __shared__ double red[32];
+    const int warps = blockDim.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < kThreads / 32; ++w) s += red[w];
+    double s = (int)(threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
 }
 
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Sums of squares, one for each block, over its share of the chunks.  The
+// bound is the reading; a square is converted and added in 64 bits (two
+// instructions for an element, at a third of the rate that the conversions
+// have), which no value of f32 can overflow.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sum_squares_kernel(const T *__restrict__ x, const __grid_constant__ Geom g,
+__global__ void __launch_bounds__(kThreads) sum_spans_kernel(const __grid_constant__ Spans<T> g, double *partial) {
+    using V = typename Vec<T>::type;
+    constexpr int VN = Vec<T>::n;
+    const uint32_t lo = (uint32_t)((uint64_t)blockIdx.x * g.chunks / gridDim.x);
+    const uint32_t hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * g.chunks / gridDim.x);
+    double s[VN] = {};
+    int k = 0;
+    for (uint32_t c = lo; c < hi; ++c) {
+        while (c >= g.first[k + 1]) ++k;
+        const T *x = g.src[k];
+        const Cut<T> cut(x, g.len[k]);
+        const V *xv = reinterpret_cast<const V *>(x + cut.head);
+        const int64_t i0 = (int64_t)(c - g.first[k]) * (kThreads * kVectors) + threadIdx.x;
+        V v[kVectors];
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u) {
+            v[u] = V{};
+            if (i0 + u * kThreads < cut.nv) v[u] = __ldg(xv + i0 + u * kThreads);
+        }
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) {
+                const double d = (double)reinterpret_cast<const T *>(&v[u])[e];
+                s[e] = fma(d, d, s[e]);
+            }
+        if (c == g.first[k]) {      // the span's edges
+            if ((int)threadIdx.x < cut.head) {
+                const double d = (double)x[threadIdx.x];
+                s[0] = fma(d, d, s[0]);
+            }
+            if ((int)threadIdx.x < cut.tail) {
+                const double d = (double)x[cut.head + cut.nv * VN + threadIdx.x];
+                s[0] = fma(d, d, s[0]);
+            }
+        }
+    }
+    double t = 0.0;
+#pragma unroll
+    for (int e = 0; e < VN; ++e) t += s[e];
+    t = block_total(t);
+    if (threadIdx.x == 0) partial[blockIdx.x] = t;
+    launch_dependents();
+}
+
+// The same for a tensor with gaps between its elements, or with several at one
+// place.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sum_strided_kernel(const T *__restrict__ x, const __grid_constant__ Geom g,
                                                                double *partial) {
     double s = 0.0;
     for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < g.count; i += (int64_t)gridDim.x * kThreads) {
@@ -62,36 +159,99 @@ __global__ void __launch_bounds__(kThreads) sum_squares_kernel(const T *__restri
     }
     s = block_total(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
+    launch_dependents();
 }
 
-// The norm and the scale from the partial sums, by one block.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const double *partial, int64_t n, double max_norm, T *norm,
-                                                        double *scale) {
+__device__ __forceinline__ double add_partials(const double *partial, int64_t n) {
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) s += partial[i];
-    s = sqrt(block_total(s));
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += partial[i];
+    return block_total(s);
+}
+
+// All partial sums by one block: their root, and (total) their sum.
+template <typename T>
+__global__ void __launch_bounds__(1024) fold_kernel(const double *partial, int64_t n, T *norm, double *total) {
+    wait_for_previous();
+    const double s = add_partials(partial, n);
     if (threadIdx.x == 0) {
-        *norm = (T)s;
-        *scale = isfinite(s) && s > max_norm ? max_norm / s : 1.0;
+        *norm = (T)sqrt(s);
+        if (total) *total = s;
+    }
+}
+
+template <typename T> __device__ __forceinline__ T scale_of(double sum, double max_norm, T *norm) {
+    const double root = sqrt(sum);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (T)root;
+    return isfinite(root) && root > max_norm ? (T)(max_norm / root) : T(1);
+}
+
+// The scaled copies.  Each block adds the partial sums for itself, in one
+// order, which costs less than another launch would, and takes its chunks last
+// to first: what the sums read last is still in the cache.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) scale_spans_kernel(const __grid_constant__ Spans<T> g,
+                                                               const __grid_constant__ Outputs<T> out,
+                                                               const double *partial, int64_t n, double max_norm,
+                                                               T *norm) {
+    using V = typename Vec<T>::type;
+    constexpr int VN = Vec<T>::n;
+    wait_for_previous();
+    const T by = scale_of<T>(add_partials(partial, n), max_norm, norm);
+    const uint32_t lo = (uint32_t)((uint64_t)blockIdx.x * g.chunks / gridDim.x);
+    const uint32_t hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * g.chunks / gridDim.x);
+    int k = g.n - 1;
+    for (uint32_t c = hi; c-- > lo;) {
+        while (c < g.first[k]) --k;
+        const T *x = g.src[k];
+        T *y = out.dst[k];
+        if (by == T(1) && x == y) continue;
+        const Cut<T> cut(x, g.len[k]);
+        const uint32_t part = c - g.first[k];
+        if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0) {
+            const V *xv = reinterpret_cast<const V *>(x + cut.head);
+            V *yv = reinterpret_cast<V *>(y + cut.head);
+            const int64_t i0 = (int64_t)part * (kThreads * kVectors) + threadIdx.x;
+            V v[kVectors];
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u)
+                if (i0 + u * kThreads < cut.nv) v[u] = xv[i0 + u * kThreads];
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u) {
+#pragma unroll
+                for (int e = 0; e < VN; ++e) reinterpret_cast<T *>(&v[u])[e] *= by;
+                if (i0 + u * kThreads < cut.nv) yv[i0 + u * kThreads] = v[u];
+            }
+            if (part == 0) {
+                if ((int)threadIdx.x < cut.head) y[threadIdx.x] = x[threadIdx.x] * by;
+                const int64_t j = cut.head + cut.nv * VN + threadIdx.x;
+                if ((int)threadIdx.x < cut.tail) y[j] = x[j] * by;
+            }
+        } else {    // the two lie differently against 16 bytes
+            const int64_t j0 = (int64_t)part * kChunk<T>;
+            const int64_t j1 = c + 1 == g.first[k + 1] ? g.len[k] : j0 + kChunk<T>;
+            for (int64_t j = j0 + threadIdx.x; j < j1; j += kThreads) y[j] = x[j] * by;
+        }
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const T *x, T *out, const __grid_constant__ Geom g,
-                                                         const double *scale) {
-    const T c = (T)*scale;
+__global__ void __launch_bounds__(kThreads) scale_strided_kernel(const T *x, T *out, const __grid_constant__ Geom g,
+                                                                 const double *partial, int64_t n, double max_norm,
+                                                                 T *norm) {
+    wait_for_previous();
+    const T by = scale_of<T>(add_partials(partial, n), max_norm, norm);
     for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < g.count; i += (int64_t)gridDim.x * kThreads) {
         int64_t so, d_o;
         offsets(g, i, so, d_o);
-        out[d_o] = x[so] * c;
+        out[d_o] = x[so] * by;
     }
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr uint64_t kPartials = 512;   // most blocks of one launch
+constexpr uint64_t kPartials = 1024;   // most blocks of one launch
+constexpr int64_t kFold = 2048;        // most partial sums that each block of the scaling adds
 
 uint64_t workspace_bytes(uint64_t count) { return (count + 1) * kPartials * sizeof(double); }
 
@@ -195,9 +355,128 @@ Geom geom(const kx_tensor *g, const kx_tensor *o) {
     return r;
 }
 
+// The offset of a nonempty tensor's lowest element from its origin, if its
+// elements fill their span, each at a place of its own; 1 if they do not.
+int64_t filled_span(const kx_tensor *t) {
+    if (is_c_contiguous(t)) return 0;
+    i128 low = 0, reach = 0;
+    for (uint32_t d = 0; d < t->rank; ++d) {
+        if (t->dims[d] == 1) continue;
+        const i128 r = (i128)t->strides[d] * (i128)(t->dims[d] - 1);
+        if (r < 0) low += r;
+        reach += r < 0 ? -r : r;
+    }
+    if (reach + 1 != (i128)numel(t->dims, t->rank) || !distinct_elements(t)) return 1;
+    return (int64_t)low;
+}
+
+bool same_strides(const kx_tensor *a, const kx_tensor *b) {
+    for (uint32_t d = 0; d < a->rank; ++d)
+        if (a->dims[d] > 1 && a->strides[d] != b->strides[d]) return false;
+    return true;
+}
+
 unsigned blocks_for(int64_t count) {
     const int64_t b = (count + kThreads * 8 - 1) / (kThreads * 8);
     return (unsigned)std::min<int64_t>((int64_t)kPartials, std::max<int64_t>(b, 1));
+}
+
+// One launch's worth of filled spans.
+template <typename T> struct Batch {
+    Spans<T> spans;
+    Outputs<T> outs;
+    unsigned blocks(const Handle *h) const {
+        return std::min<unsigned>(spans.chunks, std::min<unsigned>((unsigned)kPartials, kBlocksPerSm * h->sm_count));
+    }
+    static constexpr unsigned kBlocksPerSm = 4;
+};
+
+// A kernel that may start while the previous one ends; it waits by itself for
+// that one's results (griddepcontrol.wait).
+template <typename... Params, typename... Args>
+void launch_after(Handle *h, void (*kernel)(Params...), unsigned blocks, unsigned threads, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = h->stream;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+    ++h->launches;
+}
+
+template <typename T>
+int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_norm, const kx_tensor *outs,
+               const kx_tensor *norm, void *workspace, const char *op, kx_error *err) {
+    // which tensors are runs of memory; the rest go one by one
+    std::vector<Batch<T>> batches;
+    std::vector<uint64_t> strided;
+    for (uint64_t i = 0; i < count; ++i) {
+        const int64_t n = (int64_t)numel(grads[i].dims, grads[i].rank);
+        if (n == 0) continue;
+        const int64_t low = filled_span(&grads[i]);
+        if (low > 0 || (outs && !same_strides(&grads[i], &outs[i]))) {
+            strided.push_back(i);
+            continue;
+        }
+        if (n / kChunk<T> > (1 << 30)) return set_err(err, KX_E_UNSUPPORTED, op, "too many elements");
+        const uint32_t chunks = (uint32_t)std::max<int64_t>(1, (n + kChunk<T> - 1) / kChunk<T>);
+        if (batches.empty() || batches.back().spans.n == kSpans || batches.back().spans.chunks > (1u << 30)) {
+            batches.emplace_back();
+            batches.back().spans.n = 0;
+            batches.back().spans.chunks = 0;
+        }
+        Spans<T> &s = batches.back().spans;
+        s.src[s.n] = at<T>(&grads[i]) + low;
+        s.len[s.n] = n;
+        s.first[s.n] = s.chunks;
+        batches.back().outs.dst[s.n] = outs ? at<T>(&outs[i]) + low : nullptr;
+        s.chunks += chunks;
+        s.first[++s.n] = s.chunks;
+    }
+    double *total = static_cast<double *>(workspace), *partial = total + 1;
+    int64_t used = 0;
+    for (const Batch<T> &b : batches) {
+        sum_spans_kernel<T><<<b.blocks(h), kThreads, 0, h->stream>>>(b.spans, partial + used);
+        ++h->launches;
+        used += b.blocks(h);
+    }
+    for (uint64_t i : strided) {
+        const Geom g = geom(&grads[i], nullptr);
+        sum_strided_kernel<T><<<blocks_for(g.count), kThreads, 0, h->stream>>>(at<T>(&grads[i]), g, partial + used);
+        ++h->launches;
+        used += blocks_for(g.count);
+    }
+    T *to = at<T>(norm);
+    const double *sums = partial;
+    if (!outs || used == 0 || used > kFold) {
+        launch_after(h, fold_kernel<T>, 1, 1024, partial, used, to, outs ? total : nullptr);
+        sums = total;
+        used = 1;
+        to = nullptr;
+    }
+    if (outs) {
+        for (const Batch<T> &b : batches) {
+            launch_after(h, scale_spans_kernel<T>, b.blocks(h), kThreads, b.spans, b.outs, sums, used, max_norm, to);
+            to = nullptr;
+        }
+        for (uint64_t i : strided) {
+            const Geom g = geom(&grads[i], &outs[i]);
+            launch_after(h, scale_strided_kernel<T>, blocks_for(g.count), kThreads, at<T>(&grads[i]), at<T>(&outs[i]),
+                         g, sums, used, max_norm, to);
+            to = nullptr;
+        }
+    }
+    const cudaError_t ce = cudaGetLastError();
+    if (ce != cudaSuccess) {
+        h->cuda_fail(ce);
+        return cuda_err(err, h, op);
+    }
+    h->last_kernel = op;
+    return KX_OK;
 }
 
 template <typename T>
@@ -207,40 +486,15 @@ int norm_impl(kx_handle *hh, const kx_tensor *grads, uint64_t count, double max_
     Handle *h = &hh->impl;
     if (outs && !(std::isfinite(max_norm) && max_norm > 0.0))
         return set_err(err, KX_E_PARAM, op, "max_norm (must be finite and > 0)");
-    int rc;
     try {
-        rc = check_lists<T>(grads, count, outs, norm, workspace, bytes, op, err);
+        const int rc = check_lists<T>(grads, count, outs, norm, workspace, bytes, op, err);
+        if (rc) return rc;
+        DeviceGuard guard(h->device);
+        if (!guard.ok) return set_err(err, KX_E_NO_DEVICE, op, "cannot select device");
+        return norm_lists<T>(h, grads, count, max_norm, outs, norm, workspace, op, err);
     } catch (const std::bad_alloc &) {
-        rc = set_err(err, KX_E_PARAM, op, "out of host memory");
+        return set_err(err, KX_E_PARAM, op, "out of host memory");
     }
-    if (rc) return rc;
-    DeviceGuard guard(h->device);
-    if (!guard.ok) return set_err(err, KX_E_NO_DEVICE, op, "cannot select device");
-    double *scale = static_cast<double *>(workspace), *partial = scale + 1;
-    int64_t used = 0;
-    for (uint64_t i = 0; i < count; ++i) {
-        const Geom g = geom(&grads[i], nullptr);
-        if (g.count == 0) continue;
-        const unsigned nb = blocks_for(g.count);
-        sum_squares_kernel<T><<<nb, kThreads, 0, h->stream>>>(at<T>(&grads[i]), g, partial + used);
-        ++h->launches;
-        used += nb;
-    }
-    norm_kernel<T><<<1, kThreads, 0, h->stream>>>(partial, used, max_norm, at<T>(norm), scale);
-    ++h->launches;
-    for (uint64_t i = 0; outs && i < count; ++i) {
-        const Geom g = geom(&grads[i], &outs[i]);
-        if (g.count == 0) continue;
-        scale_kernel<T><<<blocks_for(g.count), kThreads, 0, h->stream>>>(at<T>(&grads[i]), at<T>(&outs[i]), g, scale);
-        ++h->launches;
-    }
-    const cudaError_t ce = cudaGetLastError();
-    if (ce != cudaSuccess) {
-        h->cuda_fail(ce);
-        return cuda_err(err, h, op);
-    }
-    h->last_kernel = op;
-    return KX_OK;
 }
 
 }  // namespace
