@@ -23,6 +23,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
+import struct
 import threading
 from dataclasses import dataclass, field
 from typing import NamedTuple, Sequence
@@ -219,6 +221,11 @@ def _descriptor(t) -> KxTensor:
 
 
 def _device_index(t) -> int:
+    where = getattr(t, "get_device", None)
+    if where is not None:
+        dev = where()
+        if dev >= 0:
+            return dev
     dev = t.device
     if dev.type != "cuda":
         raise NoDevice(f"expected a CUDA tensor, got {dev}")
@@ -530,16 +537,49 @@ class TokenLogProbs(NamedTuple):
     top_tokens: "object" = None         # [.., top], int64
 
 
-def _same_device(op: str, dev: int, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and _device_index(t) != dev:
-            raise InvalidParameter(f"{op}: {name} belongs to another device", operation=op, parameter=name)
+# One kx_tensor as a row of words: data, storage_len, origin, rank, then dims and
+# strides, each filled up with zeros.  These calls have many small operands
+# beside a short kernel, so their descriptors are packed, not set field by field.
+_WORDS = struct.Struct(f"={4 + MAX_RANK}Q{MAX_RANK}q")
+_PAD = [(0,) * (MAX_RANK - r) for r in range(MAX_RANK + 1)]
 
 
-def _same_dtype(op: str, dtype, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.dtype != dtype:
-            raise InvalidParameter(f"{op}: {name} is {t.dtype}, not {dtype}", operation=op, parameter=name)
+class _Operands:
+    """The descriptors of one call's operands, and where the library finds
+    them; an operand that is None has none.  Checks each one's device and
+    dtype on the way."""
+
+    def __init__(self, op: str, dev: int, count: int):
+        self.op, self.dev = op, dev
+        self.buf = C.create_string_buffer(_WORDS.size * count)
+        self.at, self.used = C.addressof(self.buf), 0
+
+    def _next(self) -> int:
+        off = self.used
+        self.used = off + _WORDS.size
+        return off
+
+    def add(self, name: str, t, dtype):
+        if t is None:
+            return None
+        if t.dtype != dtype:
+            raise InvalidParameter(f"{self.op}: {name} is {t.dtype}, not {dtype}", operation=self.op, parameter=name)
+        if _device_index(t) != self.dev:
+            raise InvalidParameter(f"{self.op}: {name} belongs to another device", operation=self.op, parameter=name)
+        if isinstance(t, TensorView) or len(t.shape) > MAX_RANK:
+            off = self._next()
+            C.memmove(self.at + off, C.byref(_descriptor(t)), _WORDS.size)
+            return self.at + off
+        if t.is_contiguous():
+            return self.put(t.data_ptr(), t.numel(), 0, t.shape, t.stride())
+        st = t.untyped_storage()
+        return self.put(st.data_ptr(), st.nbytes() // t.element_size(), t.storage_offset(), t.shape, t.stride())
+
+    def put(self, ptr: int, length: int, origin: int, dims, strides) -> int:
+        off, rank = self._next(), len(dims)
+        pad = _PAD[rank]
+        _WORDS.pack_into(self.buf, off, ptr, length, origin, rank, *dims, *pad, *strides, *pad)
+        return self.at + off
 
 
 def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int = 0,
@@ -558,19 +598,19 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
     NaN instead of raising: nothing is read back, so the call does not wait for
     the device and can be captured into a CUDA graph."""
     import torch
-    shape = tuple(logits.shape)
     top = int(top)
     if not 0 <= top <= MAX_ALTERNATIVES:
         raise InvalidParameter(f"token_log_probs: top (0 to {MAX_ALTERNATIVES} alternatives)",
                                operation="token_log_probs", parameter="top")
-    rows = shape[:-1]
-    make = lambda dims, dtype: torch.empty(dims, dtype=dtype, device=logits.device)  # noqa: E731
+    dtype, device = logits.dtype, logits.device
+    rows = tuple(logits.shape[:-1])
+    # the numbers of each row share one allocation
+    lp, lse, ent = tokens is not None, True, bool(entropy)
+    kept = iter(torch.empty((lp + lse + ent, *rows), dtype=dtype, device=device).unbind(0))
     out = TokenLogProbs(
-        log_probs=make(rows, logits.dtype) if tokens is not None else None,
-        lse=make(rows, logits.dtype),
-        entropy=make(rows, logits.dtype) if entropy else None,
-        top_log_probs=make((*rows, top), logits.dtype) if top else None,
-        top_tokens=make((*rows, top), torch.int64) if top else None)
+        log_probs=next(kept) if lp else None, lse=next(kept), entropy=next(kept) if ent else None,
+        top_log_probs=torch.empty((*rows, top), dtype=dtype, device=device) if top else None,
+        top_tokens=torch.empty((*rows, top), dtype=torch.int64, device=device) if top else None)
     token_log_probs_into(logits, tokens, out, temperature=temperature)
     return out
 
@@ -579,20 +619,17 @@ def token_log_probs_into(logits, tokens, out: TokenLogProbs, *, temperature: flo
     """``token_log_probs`` written into existing C-contiguous tensors; those
     that ``out`` holds decide what is computed."""
     import torch
-    op = "token_log_probs"
-    fn = _fn("kx_token_log_probs", logits.dtype)
+    dtype, int64 = logits.dtype, torch.int64
+    fn = _fn("kx_token_log_probs", dtype)
     h = _bind(logits)
-    _same_device(op, h.device, tokens=tokens, **out._asdict())
-    _same_dtype(op, logits.dtype, log_probs=out.log_probs, lse=out.lse, entropy=out.entropy,
-                top_log_probs=out.top_log_probs)
-    _same_dtype(op, torch.int64, tokens=tokens, top_tokens=out.top_tokens)
+    o = _Operands("token_log_probs", h.device, 7)
     err = KxError()
-    dl, dt = _ref(logits), _ref(tokens)
-    raise_for(fn(h.ptr, dl, dt, float(temperature), *[_ref(t) for t in out], C.byref(err)), err)
-
-
-def _ref(t):
-    return None if t is None else C.byref(_descriptor(t))
+    rc = fn(h.ptr, o.add("logits", logits, dtype), o.add("tokens", tokens, int64), float(temperature),
+            o.add("log_probs", out.log_probs, dtype), o.add("lse", out.lse, dtype),
+            o.add("entropy", out.entropy, dtype), o.add("top_log_probs", out.top_log_probs, dtype),
+            o.add("top_tokens", out.top_tokens, int64), C.byref(err))
+    if rc:
+        raise_for(rc, err)
 
 
 def token_log_probs_backward(logits, tokens=None, *, lse, entropy=None, grad_log_probs=None, grad_entropy=None,
@@ -604,7 +641,8 @@ def token_log_probs_backward(logits, tokens=None, *, lse, entropy=None, grad_log
     ``lse`` and (with ``grad_entropy``) ``entropy`` are the forward call's, for
     the same logits and temperature; incoming gradients have their outputs'
     dims (any strides), and one that is None counts as zero."""
-    out = _empty(tuple(logits.shape), logits.dtype, logits.device)
+    import torch
+    out = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=logits.device)
     token_log_probs_backward_into(logits, tokens, out, lse=lse, entropy=entropy, grad_log_probs=grad_log_probs,
                                   grad_entropy=grad_entropy, grad_lse=grad_lse, temperature=temperature)
     return out
@@ -614,56 +652,85 @@ def token_log_probs_backward_into(logits, tokens, out, *, lse, entropy=None, gra
                                   grad_lse=None, temperature: float = 1.0) -> None:
     """``token_log_probs_backward`` written into an existing C-contiguous tensor."""
     import torch
-    op = "token_log_probs_backward"
-    fn = _fn("kx_token_log_probs_backward", logits.dtype)
+    dtype = logits.dtype
+    fn = _fn("kx_token_log_probs_backward", dtype)
     h = _bind(logits)
-    same = dict(lse=lse, entropy=entropy, grad_log_probs=grad_log_probs, grad_entropy=grad_entropy,
-                grad_lse=grad_lse, out=out)
-    _same_device(op, h.device, tokens=tokens, **same)
-    _same_dtype(op, logits.dtype, **same)
-    _same_dtype(op, torch.int64, tokens=tokens)
+    o = _Operands("token_log_probs_backward", h.device, 8)
     err = KxError()
-    raise_for(fn(h.ptr, _ref(logits), _ref(tokens), _ref(lse), _ref(entropy), _ref(grad_log_probs),
-                 _ref(grad_entropy), _ref(grad_lse), float(temperature), _ref(out), C.byref(err)), err)
+    rc = fn(h.ptr, o.add("logits", logits, dtype), o.add("tokens", tokens, torch.int64), o.add("lse", lse, dtype),
+            o.add("entropy", entropy, dtype), o.add("grad_log_probs", grad_log_probs, dtype),
+            o.add("grad_entropy", grad_entropy, dtype), o.add("grad_lse", grad_lse, dtype), float(temperature),
+            o.add("out", out, dtype), C.byref(err))
+    if rc:
+        raise_for(rc, err)
+
+
+def _one(op: str, name: str, what: str, values, allowed=1):
+    if len(values) > allowed:
+        raise InvalidParameter(f"{op}: {name} {what}", operation=op, parameter=name)
 
 
 def _lists(op: str, grads, outs=None):
-    """The descriptors of a list of gradients (and of their outputs).  A pair of
-    C-contiguous tensors is described by its elements alone, all such pairs at
-    once: a long list's cost is in this loop."""
+    """The descriptors of a list of gradients (and of their outputs), and their
+    dtype.  Pairs of C-contiguous tensors are described by their elements
+    alone, all such pairs at once: a long list's cost is here."""
     import torch
-    grads = list(grads)
-    lists = [grads] if outs is None else [grads, list(outs)]
     if not grads:
         raise InvalidParameter(f"{op}: grads (at least one)", operation=op, parameter="grads")
-    dtype, dev = grads[0].dtype, _device_index(grads[0])
-    flat = None
-    for name, ts in zip(("grads", "outs"), lists):
+    lists = [("grads", grads)] if outs is None else [("grads", grads), ("outs", outs)]
+    first = grads[0]
+    flat = True
+    for name, ts in lists:
         if len(ts) != len(grads):
-            raise InvalidParameter(f"{op}: {len(ts)} outs for {len(grads)} grads", operation=op, parameter="outs")
-        if any(t.dtype != dtype for t in ts):
-            raise InvalidParameter(f"{op}: {name} of several dtypes", operation=op, parameter=name)
-        if any(_device_index(t) != dev for t in ts):
-            raise InvalidParameter(f"{op}: {name} on several devices", operation=op, parameter=name)
-        here = [isinstance(t, torch.Tensor) and t.is_contiguous() for t in ts]
-        flat = here if flat is None else [a and b for a, b in zip(flat, here)]
-    if outs is not None and any(tuple(g.shape) != tuple(o.shape) for g, o in zip(*lists)):
+            raise InvalidParameter(f"{op}: {len(ts)} outs for {len(grads)} grads", operation=op, parameter=name)
+        _one(op, name, "of several dtypes", {first.dtype, *[t.dtype for t in ts]})
+        if any(isinstance(t, TensorView) for t in ts):
+            devices = {_device_index(t) for t in ts}
+            flat = False
+        else:
+            devices = set(map(torch.Tensor.get_device, ts))
+            flat = flat and all(map(torch.Tensor.is_contiguous, ts))
+        if -1 in devices:
+            raise NoDevice(f"{op}: expected CUDA tensors in {name}")
+        _one(op, name, "on several devices", {_device_index(first), *devices})
+    if outs is not None and [tuple(t.shape) for t in grads] != [tuple(t.shape) for t in outs]:
         raise LayoutError(f"{op}: output shape mismatch", kind="OutputShapeMismatch")
-    return dtype, [_descriptors(ts, flat) for ts in lists]
+    if flat:
+        alone = None
+    else:
+        torch_t = [all(isinstance(t, torch.Tensor) and t.is_contiguous() for t in pair)
+                   for pair in zip(*(ts for _, ts in lists))]
+        alone = [i for i, f in enumerate(torch_t) if not f]
+    return first.dtype, [_descriptors(ts, alone) for _, ts in lists]
 
 
-def _descriptors(ts, flat):
+def _descriptors(ts, alone=None):
+    """Descriptors of C-contiguous tensors as one axis of elements each, but for
+    those at the places in ``alone``, which keep their dims and strides."""
+    import torch
     arr = (KxTensor * len(ts))()
     words = np.frombuffer(arr, dtype=np.int64).reshape(len(ts), -1)
-    counts = [t.numel() if f else 0 for t, f in zip(ts, flat)]
-    words[:, 0] = [t.data_ptr() if f else 0 for t, f in zip(ts, flat)]
-    words[:, 1] = words[:, 4] = counts      # storage_len, dims[0]
-    words[:, 3] = 1                         # rank
-    words[:, 4 + MAX_RANK] = 1              # strides[0]
-    for i, f in enumerate(flat):
-        if not f:
-            arr[i] = _descriptor(ts[i])
+    every = ts if not alone else [t if isinstance(t, torch.Tensor) else t.buffer for t in ts]
+    words[:, 0] = list(map(torch.Tensor.data_ptr, every))
+    words[:, 4] = words[:, 1] = list(map(torch.Tensor.numel, every))     # dims[0], storage_len
+    words[:, 3] = 1                                                      # rank
+    words[:, 4 + MAX_RANK] = 1                                           # strides[0]
+    for i in alone or ():
+        t = ts[i]
+        if isinstance(t, TensorView) or len(t.shape) > MAX_RANK:
+            arr[i] = _descriptor(t)
+            continue
+        st, pad = t.untyped_storage(), _PAD[len(t.shape)]
+        _WORDS.pack_into(arr, _WORDS.size * i, st.data_ptr(), st.nbytes() // t.element_size(), t.storage_offset(),
+                         len(t.shape), *t.shape, *pad, *t.stride(), *pad)
     return arr
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(count: int) -> int:
+    size = C.c_uint64()
+    raise_for(lib.kx_grad_norm_workspace(count, C.byref(size)), None)
+    return size.value
 
 
 def _norm_call(op: str, grads, outs, max_norm, norm):
@@ -671,21 +738,21 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     dtype, arrays = _lists(op, grads, outs)
     fn = _fn("kx_" + op, dtype)
     h = _bind(grads[0])
+    device = grads[0].device
     if norm is None:
-        norm = torch.empty((), dtype=dtype, device=grads[0].device)
-    _same_device(op, h.device, norm=norm)
-    _same_dtype(op, dtype, norm=norm)
-    n = len(arrays[0])
-    size = C.c_uint64()
-    raise_for(lib.kx_grad_norm_workspace(n, C.byref(size)), None)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=grads[0].device)
+        norm = torch.empty((), dtype=dtype, device=device)
+    n = len(grads)
+    size = _norm_workspace(n)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    o = _Operands(op, h.device, 1)
     err = KxError()
-    tail = (_ref(norm), ws.data_ptr(), size.value, C.byref(err))
+    tail = (o.add("norm", norm, dtype), ws.data_ptr(), size, C.byref(err))
     if outs is None:
         rc = fn(h.ptr, arrays[0], n, *tail)
     else:
         rc = fn(h.ptr, arrays[0], n, float(max_norm), arrays[1], *tail)
-    raise_for(rc, err)
+    if rc:
+        raise_for(rc, err)
     return norm
 
 

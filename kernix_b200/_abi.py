@@ -150,17 +150,15 @@ _SIGNATURES = {
                                          _P(KxTensor), _P(KxTensor), _P(KxError)]),
     "kx_conv2d_backward_f64": (C.c_int, [_vp, _P(KxTensor), _P(KxTensor), _P(KxTensor), _P(KxConv2dOptions),
                                          _P(KxTensor), _P(KxTensor), _P(KxError)]),
-    "kx_token_log_probs_f32": (C.c_int, [_vp, *[_P(KxTensor)] * 2, C.c_float, *[_P(KxTensor)] * 5, _P(KxError)]),
-    "kx_token_log_probs_f64": (C.c_int, [_vp, *[_P(KxTensor)] * 2, C.c_double, *[_P(KxTensor)] * 5, _P(KxError)]),
-    "kx_token_log_probs_backward_f32": (C.c_int, [_vp, *[_P(KxTensor)] * 7, C.c_float, _P(KxTensor), _P(KxError)]),
-    "kx_token_log_probs_backward_f64": (C.c_int, [_vp, *[_P(KxTensor)] * 7, C.c_double, _P(KxTensor), _P(KxError)]),
+    "kx_token_log_probs_f32": (C.c_int, [*[_vp] * 3, C.c_float, *[_vp] * 5, _P(KxError)]),
+    "kx_token_log_probs_f64": (C.c_int, [*[_vp] * 3, C.c_double, *[_vp] * 5, _P(KxError)]),
+    "kx_token_log_probs_backward_f32": (C.c_int, [*[_vp] * 8, C.c_float, _vp, _P(KxError)]),
+    "kx_token_log_probs_backward_f64": (C.c_int, [*[_vp] * 8, C.c_double, _vp, _P(KxError)]),
     "kx_grad_norm_workspace": (C.c_int, [_u64, _P(_u64)]),
-    "kx_grad_norm_f32": (C.c_int, [_vp, _vp, _u64, _P(KxTensor), _vp, _u64, _P(KxError)]),
-    "kx_grad_norm_f64": (C.c_int, [_vp, _vp, _u64, _P(KxTensor), _vp, _u64, _P(KxError)]),
-    "kx_clip_grad_norm_f32": (C.c_int, [_vp, _vp, _u64, C.c_double, _vp, _P(KxTensor), _vp, _u64,
-                                          _P(KxError)]),
-    "kx_clip_grad_norm_f64": (C.c_int, [_vp, _vp, _u64, C.c_double, _vp, _P(KxTensor), _vp, _u64,
-                                          _P(KxError)]),
+    "kx_grad_norm_f32": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _u64, _P(KxError)]),
+    "kx_grad_norm_f64": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _u64, _P(KxError)]),
+    "kx_clip_grad_norm_f32": (C.c_int, [_vp, _vp, _u64, C.c_double, _vp, _vp, _vp, _u64, _P(KxError)]),
+    "kx_clip_grad_norm_f64": (C.c_int, [_vp, _vp, _u64, C.c_double, _vp, _vp, _vp, _u64, _P(KxError)]),
     "kx_try_dense_matmul_f32": (C.c_int, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _u64]),
     "kx_try_dense_matmul_f64": (C.c_int, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _u64]),
     "kx_try_strided_matmul_f32": (C.c_int, [_vp, _P(KxMatrix), _P(KxMatrix), _vp, _u64]),

@@ -97,10 +97,12 @@ template <typename T> __device__ __forceinline__ T finite(T d) { return fmax(d, 
 template <typename T, bool ENT> struct Stats {
     T m = lowest<T>(), s = T(0), e = T(0);
 
-    template <int N> __device__ __forceinline__ void add(const T (&v)[N], T c) {
-        T nm = m;
+    // adds the values and gives the largest of them
+    template <int N> __device__ __forceinline__ T add(const T (&v)[N], T c) {
+        T most = lowest<T>();
 #pragma unroll
-        for (int i = 0; i < N; ++i) nm = fmax(nm, v[i]);
+        for (int i = 0; i < N; ++i) most = fmax(most, v[i]);
+        const T nm = fmax(m, most);
         // an f64 exponential costs far more than the branch around it
         if (sizeof(T) == 4 || nm != m) rebase(nm, c);
 #pragma unroll
@@ -109,6 +111,7 @@ template <typename T, bool ENT> struct Stats {
             s += p;
             if (ENT) e = fma(p, finite(d), e);
         }
+        return most;
     }
     __device__ __forceinline__ void rebase(T nm, T c) {
         const T d = m - nm, f = exp_scaled(d, c);
@@ -182,10 +185,12 @@ template <typename T> __device__ __forceinline__ T sorted_falling(T v, int lane)
 }
 
 constexpr int kCandidates = 512;
+template <int NW> constexpr int kSlots = NW == 1 ? 8 : 16;
 
 template <typename T, int NW> struct Shared {
     T m[NW], s[NW], e[NW], bound[NW];     // each warp's
     T cta_m, cta_s, cta_e;                // the block's, for its cluster
+    T slot[kSlots<NW>][NW * 32];          // each thread's maxima over parts of its elements
     int found;
     T best_v[32];                         // the block's alternatives, in order
     int best_i[32];
@@ -201,12 +206,15 @@ template <typename T, int NW> struct Shared {
 //
 // The alternatives come from the threads' maxima: the K-th largest of them, or
 // less, bounds the K-th alternative from below, so only elements at or above
-// it matter, and only the threads whose maximum reaches it read theirs again
-// (about K of them, from the cache).  A few dozen candidates are ranked by
-// counting.  Should more than kCandidates elements reach the bound (rows of
+// it matter.  Threads whose maximum reaches it (a few times K) read the parts
+// of theirs again whose own maxima do, which is one round trip to memory at
+// about 1 % of the row: going over all of their elements took 97 us where this
+// takes %FIG% (1501 x 50021 f32, 8 alternatives).  A few dozen candidates are
+// ranked by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
 template <typename T, bool VEC, bool ENT, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : NW == 1 ? 9 : 5)
+    log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
     constexpr int kRowsPerBlock = NW == 1 ? 4 : 1;
     constexpr int GT = NW * 32;           // threads that share a row in this block
     constexpr int VN = RowView<T, VEC>::VN;
@@ -243,12 +251,21 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) log_probs_kernel(cons
             const T v[1] = {lane < x.head ? x.at(lane) : T(-INFINITY)};
             st.add(v, c);
         }
+        const int rounds = (per + GT * U - 1) / (GT * U), each = (rounds + kSlots<NW> - 1) / kSlots<NW>;
+        int slots = 0, left = each;
+        T most = lowest<T>();
         for (int i = v0 + tid; i < v1; i += GT * U) {
             T v[U][VN];
 #pragma unroll
             for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
-            st.add(reinterpret_cast<T(&)[U * VN]>(v), c);
+            most = fmax(most, st.add(reinterpret_cast<T(&)[U * VN]>(v), c));
+            if (p.top > 0 && --left == 0) {
+                sh.slot[slots++][tid] = most;
+                most = lowest<T>();
+                left = each;
+            }
         }
+        if (left != each) sh.slot[slots++][tid] = most;
         if (edges) {
             const T v[1] = {lane < x.tail ? x.at(tail0 + lane) : T(-INFINITY)};
             st.add(v, c);
@@ -292,15 +309,21 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) log_probs_kernel(cons
                     }
                 }
             };
-            if (mine >= bound) {
-                for (int i = v0 + tid; i < v1; i += GT * U) {
-                    T v[U][VN];
+            if (mine >= bound && st.s != T(0)) {
+                unsigned wanted = 0;
+                for (int q = 0; q < slots; ++q) wanted |= (unsigned)(sh.slot[q][tid] >= bound) << q;
+                for (; wanted; wanted &= wanted - 1) {
+                    const int q = __ffs(wanted) - 1;
+                    for (int b = q * each; b < (q + 1) * each; ++b) {
+                        const int i = v0 + tid + b * (GT * U);
+                        T v[U][VN];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
+                        for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
+                        for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int k = 0; k < VN; ++k) offer(v[u][k], x.head + (i + u * GT) * VN + k);
+                            for (int k = 0; k < VN; ++k) offer(v[u][k], x.head + (i + u * GT) * VN + k);
+                    }
                 }
                 if (edges && lane < x.head) offer(x.at(lane), lane);
                 if (edges && lane < x.tail) offer(x.at(tail0 + lane), tail0 + lane);

@@ -219,11 +219,11 @@ def test_lists_describe_contiguous_pairs_by_their_elements():
     import torch
     g = [torch.zeros(3, 4)[1:], torch.zeros(4, 3).t(), torch.zeros(0, 3), torch.tensor(1.0), torch.zeros(2, 2)]
     o = [torch.zeros(2, 4), torch.zeros(4, 3).t(), torch.zeros(0, 3), torch.tensor(1.0), torch.zeros(2, 2).t()]
-    flat = [True, False, True, True, False]
-    arr = kx._descriptors(g, flat)
+    alone = [1, 4]
+    arr = kx._descriptors(g, alone)
     assert (arr[0].data, arr[0].rank, arr[0].dims[0], arr[0].strides[0]) == (g[0].data_ptr(), 1, 8, 1)
     assert (arr[0].storage_len, arr[0].origin) == (8, 0)
     assert (arr[1].rank, list(arr[1].dims)[:2], list(arr[1].strides)[:2]) == (2, [3, 4], [1, 3])
     assert (arr[2].rank, arr[2].dims[0]) == (1, 0) and (arr[3].rank, arr[3].dims[0]) == (1, 1)
-    arr = kx._descriptors(o, flat)
+    arr = kx._descriptors(o, alone)
     assert list(arr[4].strides)[:2] == [1, 2]
