@@ -54,7 +54,8 @@ template <typename T> struct ForwardParams {
     int64_t *top_ids;
     int64_t stride;
     int len, top, cluster;   // cluster: blocks that share a row
-    T temperature, factor;   // factor: exp_factor(temperature)
+    T factor;                // exp_factor(temperature)
+    double inverse;          // 1 / temperature
     Rows rows;
 };
 
@@ -90,6 +91,17 @@ template <> __device__ __forceinline__ double lowest<double>() { return -DBL_MAX
 // difference is -inf: their product has to be 0, not NaN.
 template <typename T> __device__ __forceinline__ T finite(T d) { return fmax(d, lowest<T>()); }
 
+__device__ __forceinline__ float warp_max(float v) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+__device__ __forceinline__ double warp_max(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 // What a thread knows of the elements that it has seen: their maximum, the sum
 // of exp((x - m)/T) and that of exp((x - m)/T) (x - m).  A NaN or +inf makes
 // the sum NaN; it stays 0 where all elements are -inf, which makes -inf the
@@ -119,14 +131,12 @@ template <typename T, bool ENT> struct Stats {
         s *= f;
         m = nm;
     }
-    // over the warp's lanes, the same in each
-    __device__ __forceinline__ void join(T c) {
-        T nm = m;
+    // over N lanes that stand side by side, the same in each; all N are one and
+    // the same in the other lanes' groups
+    template <int N> __device__ __forceinline__ void join(T c) {
+        rebase(warp_max(m), c);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) nm = fmax(nm, __shfl_xor_sync(0xffffffffu, nm, o));
-        rebase(nm, c);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
+        for (int o = N / 2; o > 0; o >>= 1) {
             s += __shfl_xor_sync(0xffffffffu, s, o);
             if (ENT) e += __shfl_xor_sync(0xffffffffu, e, o);
         }
@@ -165,10 +175,43 @@ template <typename T, bool VEC> struct RowView {
     __device__ __forceinline__ T at(int j) const { return __ldg(x + j * stride); }
 };
 
-// a before b in the order of the alternatives
-template <typename T> __device__ __forceinline__ bool before(T av, int ai, T bv, int bi) {
-    return av > bv || (av == bv && ai < bi);
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
+// An element as the alternatives are ordered: by value, then by place, the
+// lower one first.  For f32 both are one whole number, so that a comparison is
+// one too; the two zeros are equal.
+template <typename T> struct Key;
+template <> struct Key<float> {
+    uint64_t k;
+    __device__ static Key of(float v, int i) {
+        const int b = __float_as_int(v + 0.0f);
+        const uint32_t rising = (uint32_t)(b ^ ((b >> 31) & 0x7fffffff)) ^ 0x80000000u;
+        return {(uint64_t)rising << 32 | (uint32_t)~i};
+    }
+    __device__ static Key first() { return {~0ull}; }
+    __device__ static Key none() { return of(-INFINITY, INT_MAX); }
+    __device__ bool before(const Key &o) const { return k > o.k; }
+    __device__ float value() const {
+        const int b = (int)((uint32_t)(k >> 32) ^ 0x80000000u);
+        return __int_as_float(b ^ ((b >> 31) & 0x7fffffff));
+    }
+    __device__ int place() const { return (int)~(uint32_t)k; }
+    __device__ Key lane_xor(int o) const { return {__shfl_xor_sync(0xffffffffu, k, o)}; }
+};
+template <> struct __align__(16) Key<double> {
+    double v;
+    int i;
+    __device__ static Key of(double v, int i) { return {v, i}; }
+    __device__ static Key first() { return {(double)INFINITY, -1}; }
+    __device__ static Key none() { return {-(double)INFINITY, INT_MAX}; }
+    __device__ bool before(const Key &o) const { return v > o.v || (v == o.v && i < o.i); }
+    __device__ double value() const { return v; }
+    __device__ int place() const { return i; }
+    __device__ Key lane_xor(int o) const {
+        return {__shfl_xor_sync(0xffffffffu, v, o), __shfl_xor_sync(0xffffffffu, i, o)};
+    }
+};
 
 // The warp's lane values in falling order over its lanes (a bitonic network).
 template <typename T> __device__ __forceinline__ T sorted_falling(T v, int lane) {
@@ -184,24 +227,45 @@ template <typename T> __device__ __forceinline__ T sorted_falling(T v, int lane)
     return v;
 }
 
-constexpr int kCandidates = 512;
+// The same for values that rise and then fall, or the other way round.
+template <typename T> __device__ __forceinline__ T falling_again(T v, int lane) {
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) {
+        const T o = __shfl_xor_sync(0xffffffffu, v, j);
+        v = (lane & j) == 0 ? fmax(v, o) : fmin(v, o);
+    }
+    return v;
+}
+
+// The q-th largest of the warp's lane values.
+template <typename T> __device__ __forceinline__ T largest(T v, int q, int lane) {
+    if (q > 6) return __shfl_sync(0xffffffffu, sorted_falling(v, lane), q - 1);
+    for (; q > 1; --q) {
+        const unsigned at = __ballot_sync(0xffffffffu, v == warp_max(v));
+        if (lane == __ffs(at) - 1) v = T(-INFINITY);
+    }
+    return warp_max(v);
+}
+
+template <int NW> constexpr int kCandidates = NW == 1 ? 256 : 512;
+constexpr int kMaxCluster = 8;
+constexpr int kWarpTop = 12;      // alternatives for which one warp's 32 maxima bound well
 template <int NW> constexpr int kSlots = NW == 1 ? 8 : 16;
 
 template <typename T, int NW> struct Shared {
     T m[NW], s[NW], e[NW], bound[NW];     // each warp's
-    T cta_m, cta_s, cta_e;                // the block's, for its cluster
+    T part_m[kMaxCluster], part_s[kMaxCluster], part_e[kMaxCluster];    // each block's of the cluster
     T slot[kSlots<NW>][NW * 32];          // each thread's maxima over parts of its elements
     int found;
-    T best_v[32];                         // the block's alternatives, in order
-    int best_i[32];
-    T cand_v[kCandidates];
-    int cand_i[kCandidates];
+    Key<T> best[32];                      // the block's alternatives, in order
+    Key<T> cand[kCandidates<NW>];
+    Key<T> list[NW == 1 ? 1 : kMaxCluster][32];         // the alternatives of each block of the cluster
 };
 
 // The forward pass.  One pass over the logits keeps, for each thread, the
 // maximum of its elements and the two sums against it; they meet by shuffles,
-// then in shared memory, then (few rows) over the cluster's shared memory, so
-// that one launch and no workspace do for any number of rows.  The bound is
+// then in shared memory, then (few rows) in that of the cluster's first block,
+// so that one launch and no workspace do for any number of rows.  The bound is
 // the reading of the logits; the instructions for an element are about eight.
 //
 // The alternatives come from the threads' maxima: the K-th largest of them, or
@@ -231,6 +295,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
     const int C = NW == 1 ? 1 : p.cluster;
     const int rank = NW == 1 ? 0 : blockIdx.x % C;
     const T c = p.factor;
+    // the cluster's first block has to be there before the others write to it
+    if (NW > 1 && C > 1) cluster_arrive();
     const int64_t step = (int64_t)(gridDim.x / C) * kRowsPerBlock;
     for (int64_t row = (int64_t)(blockIdx.x / C) * kRowsPerBlock + (NW == 1 ? threadIdx.x >> 5 : 0);
          row < p.rows.count; row += step) {
@@ -252,6 +318,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             st.add(v, c);
         }
         const int rounds = (per + GT * U - 1) / (GT * U), each = (rounds + kSlots<NW> - 1) / kSlots<NW>;
+        const int slots_all = each > 0 ? (rounds + each - 1) / each : 0;
         int slots = 0, left = each;
         T most = lowest<T>();
         for (int i = v0 + tid; i < v1; i += GT * U) {
@@ -271,12 +338,19 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             st.add(v, c);
         }
         const T mine = st.m;
-        st.join(c);
+        st.template join<32>(c);
         T bound = lowest<T>();
-        if (p.top > 0) {
-            // NW times the (K / NW)-th largest maximum of a warp are K elements
-            const T sorted = sorted_falling(mine, lane);
-            bound = __shfl_sync(0xffffffffu, sorted, (p.top + NW - 1) / NW - 1);
+        // NW times the (K / NW)-th largest maximum of a warp are K elements
+        if (NW == 1 && p.top > kWarpTop && slots_all > 1) {
+            // of one warp's 32, the K-th would be too low: those of the parts
+            T v = sorted_falling(slots > 0 ? sh.slot[0][lane] : lowest<T>(), lane);
+            for (int q = 1; q < slots_all; ++q) {
+                const T o = sorted_falling(q < slots ? sh.slot[q][lane] : lowest<T>(), lane);
+                v = falling_again(fmax(v, __shfl_xor_sync(0xffffffffu, o, 31)), lane);
+            }
+            bound = __shfl_sync(0xffffffffu, v, p.top - 1);
+        } else if (p.top > 0) {
+            bound = largest(mine, (p.top + NW - 1) / NW, lane);
         }
         if (NW > 1) {
             if (lane == 0) {
@@ -287,10 +361,10 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             }
             if (tid == 0) sh.found = 0;
             sync();
-            st.m = lane < NW ? sh.m[lane % NW] : lowest<T>();
-            st.s = lane < NW ? sh.s[lane % NW] : T(0);
-            st.e = lane < NW ? sh.e[lane % NW] : T(0);
-            st.join(c);
+            st.m = sh.m[lane % NW];
+            st.s = sh.s[lane % NW];
+            st.e = sh.e[lane % NW];
+            st.template join<NW>(c);
             if (p.top > 0) {
 #pragma unroll
                 for (int w = 0; w < NW; ++w) bound = fmin(bound, sh.bound[w]);
@@ -303,10 +377,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             auto offer = [&](T v, int j) {
                 if (v >= bound && v > T(-INFINITY)) {
                     const int k = atomicAdd(&sh.found, 1);
-                    if (k < kCandidates) {
-                        sh.cand_v[k] = v;
-                        sh.cand_i[k] = j;
-                    }
+                    if (k < kCandidates<NW>) sh.cand[k] = Key<T>::of(v, j);
                 }
             };
             if (mine >= bound && st.s != T(0)) {
@@ -330,34 +401,22 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             }
             sync();
             const int n = sh.found;
-            if (n <= kCandidates) {
-                for (int k = tid; k < p.top; k += GT) {
-                    if (k >= n) {
-                        sh.best_v[k] = T(-INFINITY);
-                        sh.best_i[k] = INT_MAX;
-                    }
-                }
+            if (n <= kCandidates<NW>) {
+                for (int k = n + tid; k < p.top; k += GT) sh.best[k] = Key<T>::none();
                 for (int k = tid; k < n; k += GT) {
-                    const T v = sh.cand_v[k];
-                    const int j = sh.cand_i[k];
-                    int r = 0;
-                    for (int o = 0; o < n; ++o) r += before(sh.cand_v[o], sh.cand_i[o], v, j);
-                    if (r < p.top) {
-                        sh.best_v[r] = v;
-                        sh.best_i[r] = j;
-                    }
+                    const Key<T> mine_k = sh.cand[k];
+                    int place = 0;
+#pragma unroll 8
+                    for (int o = 0; o < n; ++o) place += sh.cand[o].before(mine_k);
+                    if (place < p.top) sh.best[place] = mine_k;
                 }
             } else {
-                T last_v = T(INFINITY);
-                int last_i = -1;
+                Key<T> last = Key<T>::first();
                 for (int k = 0; k < p.top; ++k) {
-                    T bv = T(-INFINITY);
-                    int bi = INT_MAX;
+                    Key<T> best = Key<T>::none();
                     auto look = [&](T v, int j) {
-                        if (before(last_v, last_i, v, j) && before(v, j, bv, bi)) {
-                            bv = v;
-                            bi = j;
-                        }
+                        const Key<T> key = Key<T>::of(v, j);
+                        if (last.before(key) && key.before(best)) best = key;
                     };
                     for (int i = v0 + tid; i < v1; i += GT) {
                         T v[VN];
@@ -369,101 +428,82 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
                     if (edges && lane < x.tail) look(x.at(tail0 + lane), tail0 + lane);
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) {
-                        const T ov = __shfl_xor_sync(0xffffffffu, bv, o);
-                        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-                        if (before(ov, oi, bv, bi)) {
-                            bv = ov;
-                            bi = oi;
-                        }
+                        const Key<T> other = best.lane_xor(o);
+                        if (other.before(best)) best = other;
                     }
                     if (NW > 1) {
                         sync();
-                        if (lane == 0) {
-                            sh.cand_v[warp] = bv;
-                            sh.cand_i[warp] = bi;
-                        }
+                        if (lane == 0) sh.cand[warp] = best;
                         sync();
 #pragma unroll
                         for (int w = 0; w < NW; ++w)
-                            if (before(sh.cand_v[w], sh.cand_i[w], bv, bi)) {
-                                bv = sh.cand_v[w];
-                                bi = sh.cand_i[w];
-                            }
+                            if (sh.cand[w].before(best)) best = sh.cand[w];
                     }
-                    if (tid == 0) {
-                        sh.best_v[k] = bv;
-                        sh.best_i[k] = bi;
-                    }
-                    last_v = bv;
-                    last_i = bi;
+                    if (tid == 0) sh.best[k] = best;
+                    last = best;
                 }
             }
             sync();
         }
-        int total = p.top;      // alternatives in best_*, in order
-        if (NW > 1 && C > 1) {
+        int total = p.top;      // alternatives in best, in order
+        if (NW > 1 && C > 1) {  // one row for the cluster, which ends with it
             cg::cluster_group cluster = cg::this_cluster();
+            Shared<T, NW> *first = cluster.map_shared_rank(&sh, 0);
+            cluster_wait();
             if (tid == 0) {
-                sh.cta_m = st.m;
-                sh.cta_s = st.s;
-                sh.cta_e = st.e;
+                first->part_m[rank] = st.m;
+                first->part_s[rank] = st.s;
+                first->part_e[rank] = st.e;
             }
-            cluster.sync();
-            if (rank == 0) {
-                const Shared<T, NW> *other = cluster.map_shared_rank(&sh, lane < C ? lane : 0);
-                st.m = lane < C ? other->cta_m : lowest<T>();
-                st.s = lane < C ? other->cta_s : T(0);
-                st.e = lane < C ? other->cta_e : T(0);
-                st.join(c);
-                if (p.top > 0) {
-                    total = C * p.top;
-                    for (int k = tid; k < total; k += GT) {
-                        const Shared<T, NW> *from = cluster.map_shared_rank(&sh, k / p.top);
-                        sh.cand_v[k] = from->best_v[k % p.top];
-                        sh.cand_i[k] = from->best_i[k % p.top];
-                    }
-                }
-            }
-            cluster.sync();     // the others' shared memory is read
-            if (rank != 0) continue;
+            if (tid < p.top) first->list[rank][tid] = sh.best[tid];
+            cluster_arrive();
+            cluster_wait();
+            if (rank != 0) return;
+            const int k = lane % kMaxCluster;
+            st.m = k < C ? sh.part_m[k] : lowest<T>();
+            st.s = k < C ? sh.part_s[k] : T(0);
+            st.e = k < C ? sh.part_e[k] : T(0);
+            st.template join<kMaxCluster>(c);
+            total = C * p.top;
         }
-        // the row's answers, in 64 bits up to their rounding
+        // the row's answers, added up in 64 bits
         const bool bad = isnan(st.s), none = st.s == T(0);
-        const double temperature = (double)p.temperature, m = (double)st.m;
-        const double log_s = none ? 0.0 : log((double)st.s);
+        const double m = (double)st.m, log_s = none ? 0.0 : (double)log(st.s);
         auto log_prob = [&](T v) {
             if (bad) return T(NAN);
             if (v == T(-INFINITY)) return T(-INFINITY);
-            return (T)(((double)v - m) / temperature - log_s);
+            return (T)fma((double)v - m, p.inverse, -log_s);
         };
         if (tid == 0) {
-            if (p.lse) p.lse[row] = bad ? T(NAN) : none ? T(-INFINITY) : (T)(m / temperature + log_s);
-            if (ENT && p.entropy) {
-                const double mean = none ? 0.0 : (double)st.e / (double)st.s / temperature;
-                p.entropy[row] = bad ? T(NAN) : (T)(log_s - mean);
-            }
+            if (p.lse) p.lse[row] = bad ? T(NAN) : none ? T(-INFINITY) : (T)fma(m, p.inverse, log_s);
+            if (ENT && p.entropy)
+                p.entropy[row] = bad ? T(NAN) : none ? T(0) : (T)fma((double)(st.e / st.s), -p.inverse, log_s);
             if (p.log_probs) p.log_probs[row] = token < 0 ? T(0) : token >= p.len ? T(NAN) : log_prob(given);
         }
         if (p.top > 0) {
             for (int k = tid; k < total; k += GT) {
-                T v = sh.best_v[k % p.top];
-                int j = sh.best_i[k % p.top], r = k;
+                Key<T> key = sh.best[k % p.top];
+                int at = k;
                 if (total > p.top) {
-                    // lists of the cluster's blocks: each in order, so the
-                    // place in them all is counted; what a list lacks stands
-                    // behind all that is there, in the order of the lists
-                    v = sh.cand_v[k];
-                    j = sh.cand_i[k];
-                    r = 0;
-                    for (int o = 0; o < total; ++o) {
-                        const T ov = sh.cand_v[o];
-                        const int oj = sh.cand_i[o];
-                        r += before(ov, oj, v, j) || (ov == v && oj == j && o < k);
+                    // the cluster's lists, in order each: how many elements of
+                    // the others come before; what a list lacks stands behind
+                    // all that is there, in the order of the lists
+                    const int own = k / p.top;
+                    at = k % p.top;
+                    key = sh.list[own][at];
+                    for (int l = 0; l < C && at < p.top; ++l) {
+                        if (l == own) continue;
+                        for (int o = 0; o < p.top; ++o) {
+                            const Key<T> other = sh.list[l][o];
+                            if (key.before(other) || (!other.before(key) && own < l)) break;
+                            ++at;
+                        }
                     }
-                    if (r >= p.top) continue;
+                    if (at >= p.top) continue;
                 }
-                p.top_lp[row * p.top + r] = log_prob(v);
-                p.top_ids[row * p.top + r] = bad || v == T(-INFINITY) ? -1 : j;
+                const T v = key.value();
+                p.top_lp[row * p.top + at] = log_prob(v);
+                p.top_ids[row * p.top + at] = bad || v == T(-INFINITY) ? -1 : key.place();
             }
         }
         sync();     // the next row's candidates overwrite these
@@ -573,7 +613,7 @@ __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const 
                 const T v[1] = {x.at(j)};
                 st.add(v, c);
             }
-            st.join(c);
+            st.template join<32>(c);
             __syncthreads();
             if ((threadIdx.x & 31) == 0) {
                 sm[threadIdx.x >> 5] = st.m;
@@ -581,9 +621,9 @@ __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const 
             }
             __syncthreads();
             const int k = threadIdx.x & 31;
-            st.m = k < NW ? sm[k % NW] : lowest<T>();
-            st.s = k < NW ? ss[k % NW] : T(0);
-            st.join(c);
+            st.m = sm[k % NW];
+            st.s = ss[k % NW];
+            st.template join<NW>(c);
             g.base = st.m;
             g.less = (T)(log((double)st.s) * unit);
         }
@@ -622,6 +662,7 @@ constexpr int64_t kMaxGrid = 1 << 30;
 constexpr int kRowWarps = 8;
 constexpr int kGradPart = 8192;   // elements of a block's part of a row in the gradient
 constexpr int kWarpRow = 2048;    // longest row that one warp takes
+constexpr int kWarpRowOfMany = 8192, kManyRows = 2048;
 
 // The temperature divides logits: it and its reciprocal are normal numbers.
 template <typename T> bool temperature_ok(T t) {
@@ -733,15 +774,18 @@ int row_output(const kx_tensor *t, const kx_tensor *logits, uint32_t es, const c
 
 template <typename T, bool VEC, bool ENT>
 void launch_forward(Handle *h, ForwardParams<T> &p) {
-    if (p.len <= kWarpRow) {
+    if (p.len <= kWarpRow || (p.len <= kWarpRowOfMany && p.rows.count >= kManyRows)) {
         const int64_t blocks = (p.rows.count + 3) / 4;
         log_probs_kernel<T, VEC, ENT, 1><<<(unsigned)std::min<int64_t>(blocks, kMaxGrid), 128, 0, h->stream>>>(p);
         h->last_kernel = "log_probs_warp";
         return;
     }
-    while (p.cluster < 8 && p.rows.count * p.cluster < 2 * h->sm_count && p.len / (2 * p.cluster) >= 4096)
+    while (p.cluster < kMaxCluster) {
+        const int64_t blocks = p.rows.count * p.cluster, piece = p.len / (2 * p.cluster);
+        if (!(blocks < h->sm_count && piece >= 4096) && !(blocks < 3 * h->sm_count && piece >= 16384)) break;
         p.cluster *= 2;
-    const int64_t rows = std::min<int64_t>(p.rows.count, kMaxGrid / p.cluster);
+    }
+    const int64_t rows = std::min<int64_t>(p.rows.count, kMaxGrid);    // all of them where there is a cluster
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * p.cluster));
     cfg.blockDim = dim3(kRowWarps * 32);
@@ -820,7 +864,7 @@ int forward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *tokens
     p.len = (int)logits->dims[logits->rank - 1];
     p.stride = logits->strides[logits->rank - 1];
     p.top = (int)top;
-    p.temperature = temperature;
+    p.inverse = 1.0 / (double)temperature;
     p.factor = exp_factor<T>(temperature);
     p.cluster = 1;
     DeviceGuard guard(h->device);
