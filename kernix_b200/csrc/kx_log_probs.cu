@@ -69,27 +69,76 @@ template <> struct Vec<double> {
     static constexpr int n = 2;
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
+// Exponentials of differences d = x - m <= 0.  They take d c, c = unit / T.
+//
+// f32: 2^a by the special-function unit, whose few half steps of error are
+// below those of the difference itself; results under the smallest normal
+// number are 0.
+//
+// f64: a counts sixteenths, 2^(a/16).  With n = round(a) and g = a - n, which
+// is exact, it is 2^(n/16) 2^(g/16): the first factor is one of 16 roots with n's
+// whole part in its exponent, the second 1 + g q(g), |g| <= 1/2, from the
+// Taylor series of 2^x to the seventh power (the eighth is below 2^-59).  That
+// is 12 operations in 64 bits instead of the about 25 of exp(), which with its
+// registers held the f64 pass over the logits at a third of its speed.
+// Below 2^-1020 nothing counts: neither in a sum beside exp(0) nor after
+// multiplication with the difference, which may be -inf there.
+template <typename T> struct Exp;
 
-// exp((x - m)/T) of a difference d = x - m <= 0.  f32: 2^(d c), c = log2(e)/T,
-// by the special-function unit, whose few half steps of error are below those
-// of the difference itself; results under the smallest normal number are 0.
-__device__ __forceinline__ float exp_scaled(float d, float c) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * c));
-    return e;
+// 1.5 2^52, which leaves a sum's last place at 1, and log(2)^i / i! / 16^i from
+// the seventh down: in constant memory an instruction takes them as they are,
+// where 64-bit literals take two more instructions each.
+__constant__ double kExpTerms[8] = {6755399441055744.0,
+                                    0.000015252733804059840280 / 268435456,
+                                    0.00015403530393381609954 / 16777216,
+                                    0.0013333558146428443423 / 1048576,
+                                    0.0096181291076284771620 / 65536,
+                                    0.055504108664821579953 / 4096,
+                                    0.24022650695910071233 / 256,
+                                    0.69314718055994530942 / 16};
+
+template <> struct Exp<float> {
+    static constexpr double unit = 1.4426950408889634;      // log2(e)
+    struct Table {};
+    __device__ __forceinline__ explicit Exp(const Table &) {}
+    __device__ __forceinline__ float operator()(float a) const {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a));
+        return e;
+    }
+};
+template <> struct Exp<double> {
+    static constexpr double unit = 16 * 1.4426950408889634074;
+    struct Table {
+        double root[16];    // 2^(j/16)
+    };
+    const double *root;
+    __device__ __forceinline__ explicit Exp(const Table &t) : root(t.root) {}
+    __device__ __forceinline__ static bool counts(double a) { return !(a < -16.0 * 1020.0); }   // a NaN does
+    __device__ __forceinline__ double operator()(double a) const {
+        const double shifted = a + kExpTerms[0], g = a - (shifted - kExpTerms[0]);
+        const int n = __double2loint(shifted);
+        const double r = root[n & 15];
+        const double scaled = __hiloint2double(__double2hiint(r) + ((n >> 4) << 20), __double2loint(r));
+        double q = fma(kExpTerms[1], g, kExpTerms[2]);
+#pragma unroll
+        for (int i = 3; i < 8; ++i) q = fma(q, g, kExpTerms[i]);
+        return fma(scaled, q * g, scaled);
+    }
+};
+// The first threads of a block or warp fill the table; a barrier follows.
+__device__ __forceinline__ void fill(Exp<float>::Table &, int) {}
+__device__ __forceinline__ void fill(Exp<double>::Table &t, int tid) {
+    if (tid < 16) t.root[tid] = exp2((double)tid / 16);
 }
-__device__ __forceinline__ double exp_scaled(double d, double c) { return exp(d * c); }
-template <typename T> T exp_factor(T temperature);
-template <> float exp_factor<float>(float t) { return kLog2e / t; }
-template <> double exp_factor<double>(double t) { return 1.0 / t; }
+template <typename T> T exp_factor(T temperature) { return (T)(Exp<T>::unit / (double)temperature); }
 
 template <typename T> __device__ __forceinline__ T lowest();
 template <> __device__ __forceinline__ float lowest<float>() { return -FLT_MAX; }
 template <> __device__ __forceinline__ double lowest<double>() { return -DBL_MAX; }
-// A difference before it is multiplied by its exponential, which is 0 if the
-// difference is -inf: their product has to be 0, not NaN.
-template <typename T> __device__ __forceinline__ T finite(T d) { return fmax(d, lowest<T>()); }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+// no instruction has it in 64 bits; b where a is NaN
+__device__ __forceinline__ double larger(double a, double b) { return a > b ? a : b; }
 
 __device__ __forceinline__ float warp_max(float v) {
     float m;
@@ -98,7 +147,7 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 __device__ __forceinline__ double warp_max(double v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
@@ -110,31 +159,42 @@ template <typename T, bool ENT> struct Stats {
     T m = lowest<T>(), s = T(0), e = T(0);
 
     // adds the values and gives the largest of them
-    template <int N> __device__ __forceinline__ T add(const T (&v)[N], T c) {
+    template <int N> __device__ __forceinline__ T add(const T (&v)[N], T c, const Exp<T> &ex) {
         T most = lowest<T>();
 #pragma unroll
-        for (int i = 0; i < N; ++i) most = fmax(most, v[i]);
-        const T nm = fmax(m, most);
-        // an f64 exponential costs far more than the branch around it
-        if (sizeof(T) == 4 || nm != m) rebase(nm, c);
+        for (int i = 0; i < N; ++i) most = larger(v[i], most);
+        const T nm = larger(most, m);
+        // one more f32 exponential costs less than a branch around it
+        if (sizeof(T) == 4 || nm != m) rebase(nm, c, ex);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const T d = v[i] - m, p = exp_scaled(d, c);
-            s += p;
-            if (ENT) e = fma(p, finite(d), e);
+            const T d = v[i] - m;
+            if constexpr (sizeof(T) == 4) {
+                const T p = ex(d * c);
+                s += p;
+                // of a difference of -inf the exponential is 0, and so is the product
+                if (ENT) e = fma(p, larger(d, lowest<T>()), e);
+            } else if (Exp<T>::counts(d * c)) {
+                const T p = ex(d * c);
+                s += p;
+                if (ENT) e = fma(p, d, e);
+            }
         }
         return most;
     }
-    __device__ __forceinline__ void rebase(T nm, T c) {
-        const T d = m - nm, f = exp_scaled(d, c);
+    __device__ __forceinline__ void rebase(T nm, T c, const Exp<T> &ex) {
+        const T d = m - nm;
+        T f;
+        if constexpr (sizeof(T) == 4) f = ex(d * c);
+        else f = Exp<T>::counts(d * c) ? ex(d * c) : T(0);
         if (ENT) e = f == T(0) ? T(0) : fma(d, s, e) * f;
         s *= f;
         m = nm;
     }
     // over N lanes that stand side by side, the same in each; all N are one and
     // the same in the other lanes' groups
-    template <int N> __device__ __forceinline__ void join(T c) {
-        rebase(warp_max(m), c);
+    template <int N> __device__ __forceinline__ void join(T c, const Exp<T> &ex) {
+        rebase(warp_max(m), c, ex);
 #pragma unroll
         for (int o = N / 2; o > 0; o >>= 1) {
             s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -256,6 +316,7 @@ template <typename T, int NW> struct Shared {
     T m[NW], s[NW], e[NW], bound[NW];     // each warp's
     T part_m[kMaxCluster], part_s[kMaxCluster], part_e[kMaxCluster];    // each block's of the cluster
     T slot[kSlots<NW>][NW * 32];          // each thread's maxima over parts of its elements
+    typename Exp<T>::Table table;
     int found;
     Key<T> best[32];                      // the block's alternatives, in order
     Key<T> cand[kCandidates<NW>];
@@ -277,7 +338,7 @@ template <typename T, int NW> struct Shared {
 // ranked by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
 template <typename T, bool VEC, bool ENT, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : NW == 1 ? 9 : 5)
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW == 1 ? 5 : 3) : NW == 1 ? 9 : 5)
     log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
     constexpr int kRowsPerBlock = NW == 1 ? 4 : 1;
     constexpr int GT = NW * 32;           // threads that share a row in this block
@@ -295,6 +356,11 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
     const int C = NW == 1 ? 1 : p.cluster;
     const int rank = NW == 1 ? 0 : blockIdx.x % C;
     const T c = p.factor;
+    const Exp<T> ex(sh.table);
+    if (sizeof(T) == 8) {
+        fill(sh.table, tid);
+        sync();
+    }
     // the cluster's first block has to be there before the others write to it
     if (NW > 1 && C > 1) cluster_arrive();
     const int64_t step = (int64_t)(gridDim.x / C) * kRowsPerBlock;
@@ -315,7 +381,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
         Stats<T, ENT> st;
         if (edges) {
             const T v[1] = {lane < x.head ? x.at(lane) : T(-INFINITY)};
-            st.add(v, c);
+            st.add(v, c, ex);
         }
         const int rounds = (per + GT * U - 1) / (GT * U), each = (rounds + kSlots<NW> - 1) / kSlots<NW>;
         const int slots_all = each > 0 ? (rounds + each - 1) / each : 0;
@@ -325,7 +391,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             T v[U][VN];
 #pragma unroll
             for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
-            most = fmax(most, st.add(reinterpret_cast<T(&)[U * VN]>(v), c));
+            most = fmax(most, st.add(reinterpret_cast<T(&)[U * VN]>(v), c, ex));
             if (p.top > 0 && --left == 0) {
                 sh.slot[slots++][tid] = most;
                 most = lowest<T>();
@@ -335,10 +401,10 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
         if (left != each) sh.slot[slots++][tid] = most;
         if (edges) {
             const T v[1] = {lane < x.tail ? x.at(tail0 + lane) : T(-INFINITY)};
-            st.add(v, c);
+            st.add(v, c, ex);
         }
         const T mine = st.m;
-        st.template join<32>(c);
+        st.template join<32>(c, ex);
         T bound = lowest<T>();
         // NW times the (K / NW)-th largest maximum of a warp are K elements
         if (NW == 1 && p.top > kWarpTop && slots_all > 1) {
@@ -346,7 +412,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             T v = sorted_falling(slots > 0 ? sh.slot[0][lane] : lowest<T>(), lane);
             for (int q = 1; q < slots_all; ++q) {
                 const T o = sorted_falling(q < slots ? sh.slot[q][lane] : lowest<T>(), lane);
-                v = falling_again(fmax(v, __shfl_xor_sync(0xffffffffu, o, 31)), lane);
+                v = falling_again(larger(v, __shfl_xor_sync(0xffffffffu, o, 31)), lane);
             }
             bound = __shfl_sync(0xffffffffu, v, p.top - 1);
         } else if (p.top > 0) {
@@ -364,7 +430,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             st.m = sh.m[lane % NW];
             st.s = sh.s[lane % NW];
             st.e = sh.e[lane % NW];
-            st.template join<NW>(c);
+            st.template join<NW>(c, ex);
             if (p.top > 0) {
 #pragma unroll
                 for (int w = 0; w < NW; ++w) bound = fmin(bound, sh.bound[w]);
@@ -463,7 +529,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? 2 : 
             st.m = k < C ? sh.part_m[k] : lowest<T>();
             st.s = k < C ? sh.part_s[k] : T(0);
             st.e = k < C ? sh.part_e[k] : T(0);
-            st.template join<kMaxCluster>(c);
+            st.template join<kMaxCluster>(c, ex);
             total = C * p.top;
         }
         // the row's answers, added up in 64 bits
@@ -516,7 +582,8 @@ template <typename T> struct BackwardParams {
     T *out;
     int64_t stride;
     int len, per, parts;     // elements of one block's part of a row; parts of a row
-    T temperature, factor;
+    T factor;                // exp_factor(temperature)
+    double temperature, inverse;
     Rows rows;
 };
 
@@ -525,37 +592,32 @@ template <typename T> struct BackwardParams {
 // anew instead.
 constexpr double kLseTrusted = 256.0;
 
-// log p as the exponential below takes it: in units of log 2 for f32.
-constexpr double kUnit32 = 1.4426950408889634;
-template <typename T> __device__ __forceinline__ double log_unit() { return sizeof(T) == 4 ? kUnit32 : 1.0; }
-__device__ __forceinline__ float exp_unit(float a) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a));
-    return e;
-}
-__device__ __forceinline__ double exp_unit(double a) { return exp(a); }
-
 // A row's numbers in the gradient of its elements:
-//   log p = (x - base) c - less,  dx = p (a - b log p)  [+ at the token]
+//   l = (x - base) c - less, which is log p in the exponential's units,
+//   dx = p (a - b l)  [+ at the token]
 template <typename T> struct RowGrad {
     T base, less, a, b, at_token;
     int token;
-    __device__ __forceinline__ T operator()(T v, T c) const {
-        const T lq = fma(v - base, c, -less);
-        const T d = exp_unit(lq) * fma(-b, fmax(lq, T(-1e5)), a);
-        return v == T(-INFINITY) ? T(0) : d;
+    __device__ __forceinline__ T operator()(T v, T c, const Exp<T> &ex) const {
+        const T l = fma(v - base, c, -less);
+        if constexpr (sizeof(T) == 4) {
+            const T d = ex(l) * fma(-b, larger(l, T(-1e5)), a);
+            return v == T(-INFINITY) ? T(0) : d;
+        } else {
+            return Exp<T>::counts(l) ? ex(l) * fma(-b, l, a) : T(0);
+        }
     }
 };
 
 // Elements lo to hi of the row whose logits x walks and whose gradient is out.
 template <typename T, bool VEC, int THREADS>
 __device__ __forceinline__ void grad_part(const RowView<T, VEC> &x, T *out, int lo, int hi, const RowGrad<T> &g, T c,
-                                          bool first, bool last) {
+                                          const Exp<T> &ex, bool first, bool last) {
     constexpr int VN = RowView<T, VEC>::VN;
     constexpr int U = VEC ? 4 : 8;
     auto one = [&](int j) {
         const T v = x.at(j);
-        T d = g(v, c);
+        T d = g(v, c, ex);
         if (j == g.token && v != T(-INFINITY)) d += g.at_token;
         out[j] = d;
     };
@@ -568,7 +630,7 @@ __device__ __forceinline__ void grad_part(const RowView<T, VEC> &x, T *out, int 
             const int j = x.head + (i + u * THREADS) * VN;
             T d[VN];
 #pragma unroll
-            for (int k = 0; k < VN; ++k) d[k] = g(v[u][k], c);
+            for (int k = 0; k < VN; ++k) d[k] = g(v[u][k], c, ex);
             if ((unsigned)(g.token - j) < (unsigned)VN) {
 #pragma unroll
                 for (int k = 0; k < VN; ++k)
@@ -592,28 +654,34 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
     constexpr int NW = kGradThreads / 32;
     __shared__ T sm[NW], ss[NW];
+    __shared__ typename Exp<T>::Table table;
+    const Exp<T> ex(table);
+    if (sizeof(T) == 8) {
+        fill(table, threadIdx.x);
+        __syncthreads();
+    }
     const T c = p.factor;
     const int64_t total = p.rows.count * p.parts;
     for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int64_t row = w / p.parts;
+        const int64_t row = w >> 32 ? w / p.parts : (uint32_t)w / (uint32_t)p.parts;
         const int part = (int)(w - row * p.parts);
         const T *xr = p.x + row_offset(p.rows, kLogits, row);
         T *out = p.out + row * p.len;
         const double lse = (double)p.lse[row_offset(p.rows, kLse, row)];
-        const double temperature = (double)p.temperature, unit = log_unit<T>();
+        const double unit = Exp<T>::unit;
         RowGrad<T> g;
         if (fabs(lse) <= kLseTrusted) {
-            const double b = lse * temperature;
+            const double b = lse * p.temperature;
             g.base = (T)b;
-            g.less = (T)((b - (double)g.base) / temperature * unit);
+            g.less = (T)((b - (double)g.base) * (p.inverse * unit));
         } else {
             const RowView<T, VEC> x(xr, p.len, p.stride);
             Stats<T, false> st;
             for (int j = threadIdx.x; j < p.len; j += kGradThreads) {
                 const T v[1] = {x.at(j)};
-                st.add(v, c);
+                st.add(v, c, ex);
             }
-            st.template join<32>(c);
+            st.template join<32>(c, ex);
             __syncthreads();
             if ((threadIdx.x & 31) == 0) {
                 sm[threadIdx.x >> 5] = st.m;
@@ -623,9 +691,9 @@ __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const 
             const int k = threadIdx.x & 31;
             st.m = sm[k % NW];
             st.s = ss[k % NW];
-            st.template join<NW>(c);
+            st.template join<NW>(c, ex);
             g.base = st.m;
-            g.less = (T)(log((double)st.s) * unit);
+            g.less = st.s == T(0) ? T(0) : (T)(log((double)st.s) * unit);
         }
         const int64_t t = p.tokens ? p.tokens[row_offset(p.rows, kTokens, row)] : -1;
         T gp = p.g_lp && t >= 0 ? p.g_lp[row_offset(p.rows, kGradLp, row)] : T(0);
@@ -633,9 +701,9 @@ __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const 
         const T gh = p.g_h ? p.g_h[row_offset(p.rows, kGradH, row)] : T(0);
         const T h = p.g_h ? p.entropy[row_offset(p.rows, kEntropy, row)] : T(0);
         const T gl = p.g_lse ? p.g_lse[row_offset(p.rows, kGradLse, row)] : T(0);
-        g.a = (gl - gp - gh * h) / p.temperature;
-        g.b = (T)((double)gh / temperature / unit);
-        g.at_token = gp / p.temperature;
+        g.a = (T)((double)(gl - gp - gh * h) * p.inverse);
+        g.b = (T)((double)gh * (p.inverse / unit));
+        g.at_token = (T)((double)gp * p.inverse);
         g.token = t >= 0 && t < p.len ? (int)t : -1;
         // vectors where logits and gradient lie alike against 16 bytes
         const bool alike = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
@@ -643,11 +711,11 @@ __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const 
             const RowView<T, true> x(xr, p.len, p.stride);
             const int per = p.per / RowView<T, true>::VN;
             const int lo = min(part * per, x.nv), hi = part + 1 == p.parts ? x.nv : min(lo + per, x.nv);
-            grad_part<T, true, kGradThreads>(x, out, lo, hi, g, c, part == 0, part + 1 == p.parts);
+            grad_part<T, true, kGradThreads>(x, out, lo, hi, g, c, ex, part == 0, part + 1 == p.parts);
         } else {
             const RowView<T, false> x(xr, p.len, p.stride);
             const int lo = min(part * p.per, p.len), hi = part + 1 == p.parts ? p.len : min(lo + p.per, p.len);
-            grad_part<T, false, kGradThreads>(x, out, lo, hi, g, c, false, false);
+            grad_part<T, false, kGradThreads>(x, out, lo, hi, g, c, ex, false, false);
         }
     }
 }
@@ -944,7 +1012,8 @@ int backward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *token
     p.out = at<T>(grad_logits);
     p.len = (int)logits->dims[logits->rank - 1];
     p.stride = logits->strides[logits->rank - 1];
-    p.temperature = temperature;
+    p.temperature = (double)temperature;
+    p.inverse = 1.0 / (double)temperature;
     p.factor = exp_factor<T>(temperature);
     p.per = kGradPart;
     p.parts = std::max(1, (p.len + p.per - 1) / p.per);
