@@ -174,10 +174,12 @@ template <typename T, bool ENT> struct Stats {
                 s += p;
                 // of a difference of -inf the exponential is 0, and so is the product
                 if (ENT) e = fma(p, larger(d, lowest<T>()), e);
-            } else if (Exp<T>::counts(d * c)) {
-                const T p = ex(d * c);
-                s += p;
-                if (ENT) e = fma(p, d, e);
+            } else {
+                const T p = ex(d * c);      // and thrown away, rather than a branch for each
+                if (Exp<T>::counts(d * c)) {
+                    s += p;
+                    if (ENT) e = fma(p, d, e);
+                }
             }
         }
         return most;
@@ -338,7 +340,7 @@ template <typename T, int NW> struct Shared {
 // ranked by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
 template <typename T, bool VEC, bool ENT, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW == 1 ? 5 : 3) : NW == 1 ? 9 : 5)
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW == 1 ? 5 : 4) : NW == 1 ? 9 : 5)
     log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
     constexpr int kRowsPerBlock = NW == 1 ? 4 : 1;
     constexpr int GT = NW * 32;           // threads that share a row in this block
@@ -609,50 +611,115 @@ template <typename T> struct RowGrad {
     }
 };
 
-// Elements lo to hi of the row whose logits x walks and whose gradient is out.
-template <typename T, bool VEC, int THREADS>
-__device__ __forceinline__ void grad_part(const RowView<T, VEC> &x, T *out, int lo, int hi, const RowGrad<T> &g, T c,
-                                          const Exp<T> &ex, bool first, bool last) {
-    constexpr int VN = RowView<T, VEC>::VN;
-    constexpr int U = VEC ? 4 : 8;
-    auto one = [&](int j) {
-        const T v = x.at(j);
-        T d = g(v, c, ex);
-        if (j == g.token && v != T(-INFINITY)) d += g.at_token;
-        out[j] = d;
-    };
-    for (int i = lo + (int)threadIdx.x; i < hi; i += THREADS * U) {
-        T v[U][VN];
+// The vectors lo to hi (one by one without VEC) of a row, by GT threads, first
+// the loads of a thread's first round, then everything else: the row's own
+// numbers come from memory meanwhile.
+template <typename T, bool VEC, int GT> struct GradPart {
+    static constexpr int VN = RowView<T, VEC>::VN;
+    static constexpr int U = VEC ? 4 : 64 / (int)sizeof(T);   // 64 bytes in flight for each thread
+    T v[U][VN];
+    const int lo, hi, tid;
+
+    __device__ __forceinline__ GradPart(const RowView<T, VEC> &x, int lo_, int hi_, int tid_)
+        : lo(lo_), hi(hi_), tid(tid_) {
+        load(x, lo + tid);
+    }
+    __device__ __forceinline__ void load(const RowView<T, VEC> &x, int i) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) x.load(i + u * THREADS, i + u * THREADS < hi, v[u]);
+        for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < hi, v[u]);
+    }
+    __device__ __forceinline__ void run(const RowView<T, VEC> &x, T *out, const RowGrad<T> &g, T c, const Exp<T> &ex,
+                                        bool first, bool last) {
+        for (int i = lo + tid; i < hi; i += GT * U) {
+            if (i != lo + tid) load(x, i);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = x.head + (i + u * THREADS) * VN;
-            T d[VN];
+            for (int u = 0; u < U; ++u) {
+                const int j = x.head + (i + u * GT) * VN;
+                T d[VN];
 #pragma unroll
-            for (int k = 0; k < VN; ++k) d[k] = g(v[u][k], c, ex);
-            if ((unsigned)(g.token - j) < (unsigned)VN) {
+                for (int k = 0; k < VN; ++k) d[k] = g(v[u][k], c, ex);
+                if ((unsigned)(g.token - j) < (unsigned)VN) {
 #pragma unroll
-                for (int k = 0; k < VN; ++k)
-                    if (g.token == j + k && v[u][k] != T(-INFINITY)) d[k] += g.at_token;
-            }
-            if (i + u * THREADS < hi) {
-                if (VEC) *reinterpret_cast<typename Vec<T>::type *>(out + j) = *reinterpret_cast<const typename Vec<T>::type *>(d);
-                else out[j] = d[0];
+                    for (int k = 0; k < VN; ++k)
+                        if (g.token == j + k && v[u][k] != T(-INFINITY)) d[k] += g.at_token;
+                }
+                if (i + u * GT < hi) {
+                    if (VEC)
+                        *reinterpret_cast<typename Vec<T>::type *>(out + j) =
+                            *reinterpret_cast<const typename Vec<T>::type *>(d);
+                    else
+                        out[j] = d[0];
+                }
             }
         }
+        if (VEC && first && tid < x.head) one(x, out, tid, g, c, ex);
+        if (VEC && last && tid < x.tail) one(x, out, x.head + x.nv * VN + tid, g, c, ex);
     }
-    if (VEC && first && (int)threadIdx.x < x.head) one(threadIdx.x);
-    if (VEC && last && (int)threadIdx.x < x.tail) one(x.head + x.nv * VN + threadIdx.x);
+    __device__ __forceinline__ static void one(const RowView<T, VEC> &x, T *out, int j, const RowGrad<T> &g, T c,
+                                               const Exp<T> &ex) {
+        const T value = x.at(j);
+        T d = g(value, c, ex);
+        if (j == g.token && value != T(-INFINITY)) d += g.at_token;
+        out[j] = d;
+    }
+};
+
+constexpr int kGradThreads = 256, kGradBlocks = 4;    // threads of a block, blocks of an SM
+
+// A row's numbers for its gradient, by the NW warps that share it.
+template <typename T, int NW>
+__device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64_t row, const T *xr, int tid, T *sm,
+                                               T *ss, const Exp<T> &ex) {
+    const double unit = Exp<T>::unit;
+    const double lse = (double)p.lse[row_offset(p.rows, kLse, row)];
+    const int64_t t = p.tokens ? p.tokens[row_offset(p.rows, kTokens, row)] : -1;
+    T gp = p.g_lp ? p.g_lp[row_offset(p.rows, kGradLp, row)] : T(0);
+    const T gh = p.g_h ? p.g_h[row_offset(p.rows, kGradH, row)] : T(0);
+    const T h = p.g_h ? p.entropy[row_offset(p.rows, kEntropy, row)] : T(0);
+    const T gl = p.g_lse ? p.g_lse[row_offset(p.rows, kGradLse, row)] : T(0);
+    RowGrad<T> g;
+    if (fabs(lse) <= kLseTrusted) {
+        const double b = lse * p.temperature;
+        g.base = (T)b;
+        g.less = (T)((b - (double)g.base) * (p.inverse * unit));
+    } else {
+        Stats<T, false> st;
+        for (int j = tid; j < p.len; j += NW * 32) {
+            const T v[1] = {__ldg(xr + j * p.stride)};
+            st.add(v, p.factor, ex);
+        }
+        st.template join<32>(p.factor, ex);
+        if (NW > 1) {
+            __syncthreads();
+            if ((tid & 31) == 0) {
+                sm[tid >> 5] = st.m;
+                ss[tid >> 5] = st.s;
+            }
+            __syncthreads();
+            st.m = sm[tid % NW];
+            st.s = ss[tid % NW];
+            st.template join<NW>(p.factor, ex);
+        }
+        g.base = st.m;
+        g.less = st.s == T(0) ? T(0) : (T)(log((double)st.s) * unit);
+    }
+    if (t < 0) gp = T(0);
+    if (t >= p.len) gp = T(NAN);
+    g.a = (T)((double)(gl - gp - gh * h) * p.inverse);
+    g.b = (T)((double)gh * (p.inverse / unit));
+    g.at_token = (T)((double)gp * p.inverse);
+    g.token = t >= 0 && t < p.len ? (int)t : -1;
+    return g;
 }
 
-constexpr int kGradThreads = 256;
-
 // The gradient: one element in, one out, with a row's few numbers between
-// them.  The bound is the two streams; a block takes a part of one row.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
-    constexpr int NW = kGradThreads / 32;
+// them.  The bound is the two streams.  A block takes a part of one row (long
+// parts where there are many rows: 4096 x 32000 f32 in parts of %G1%), or each
+// of its warps a short row.
+template <typename T, bool VEC, int NW>
+__global__ void __launch_bounds__(kGradThreads, kGradBlocks) log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
+    constexpr int GT = NW * 32;
+    constexpr int kGroups = kGradThreads / GT;
     __shared__ T sm[NW], ss[NW];
     __shared__ typename Exp<T>::Table table;
     const Exp<T> ex(table);
@@ -660,62 +727,27 @@ __global__ void __launch_bounds__(kGradThreads) log_probs_backward_kernel(const 
         fill(table, threadIdx.x);
         __syncthreads();
     }
-    const T c = p.factor;
+    const int tid = threadIdx.x % GT;
     const int64_t total = p.rows.count * p.parts;
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+    for (int64_t w = (int64_t)blockIdx.x * kGroups + threadIdx.x / GT; w < total; w += (int64_t)gridDim.x * kGroups) {
         const int64_t row = w >> 32 ? w / p.parts : (uint32_t)w / (uint32_t)p.parts;
         const int part = (int)(w - row * p.parts);
         const T *xr = p.x + row_offset(p.rows, kLogits, row);
         T *out = p.out + row * p.len;
-        const double lse = (double)p.lse[row_offset(p.rows, kLse, row)];
-        const double unit = Exp<T>::unit;
-        RowGrad<T> g;
-        if (fabs(lse) <= kLseTrusted) {
-            const double b = lse * p.temperature;
-            g.base = (T)b;
-            g.less = (T)((b - (double)g.base) * (p.inverse * unit));
-        } else {
-            const RowView<T, VEC> x(xr, p.len, p.stride);
-            Stats<T, false> st;
-            for (int j = threadIdx.x; j < p.len; j += kGradThreads) {
-                const T v[1] = {x.at(j)};
-                st.add(v, c, ex);
-            }
-            st.template join<32>(c, ex);
-            __syncthreads();
-            if ((threadIdx.x & 31) == 0) {
-                sm[threadIdx.x >> 5] = st.m;
-                ss[threadIdx.x >> 5] = st.s;
-            }
-            __syncthreads();
-            const int k = threadIdx.x & 31;
-            st.m = sm[k % NW];
-            st.s = ss[k % NW];
-            st.template join<NW>(c, ex);
-            g.base = st.m;
-            g.less = st.s == T(0) ? T(0) : (T)(log((double)st.s) * unit);
-        }
-        const int64_t t = p.tokens ? p.tokens[row_offset(p.rows, kTokens, row)] : -1;
-        T gp = p.g_lp && t >= 0 ? p.g_lp[row_offset(p.rows, kGradLp, row)] : T(0);
-        if (t >= p.len) gp = T(NAN);
-        const T gh = p.g_h ? p.g_h[row_offset(p.rows, kGradH, row)] : T(0);
-        const T h = p.g_h ? p.entropy[row_offset(p.rows, kEntropy, row)] : T(0);
-        const T gl = p.g_lse ? p.g_lse[row_offset(p.rows, kGradLse, row)] : T(0);
-        g.a = (T)((double)(gl - gp - gh * h) * p.inverse);
-        g.b = (T)((double)gh * (p.inverse / unit));
-        g.at_token = (T)((double)gp * p.inverse);
-        g.token = t >= 0 && t < p.len ? (int)t : -1;
+        const bool first = part == 0, last = part + 1 == p.parts;
         // vectors where logits and gradient lie alike against 16 bytes
-        const bool alike = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-        if (VEC && alike) {
+        if (VEC && ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
             const RowView<T, true> x(xr, p.len, p.stride);
-            const int per = p.per / RowView<T, true>::VN;
-            const int lo = min(part * per, x.nv), hi = part + 1 == p.parts ? x.nv : min(lo + per, x.nv);
-            grad_part<T, true, kGradThreads>(x, out, lo, hi, g, c, ex, part == 0, part + 1 == p.parts);
+            const int per = p.per / RowView<T, true>::VN, lo = min(part * per, x.nv);
+            GradPart<T, true, GT> g(x, lo, last ? x.nv : min(lo + per, x.nv), tid);
+            const RowGrad<T> numbers = row_grad<T, NW>(p, row, xr, tid, sm, ss, ex);
+            g.run(x, out, numbers, p.factor, ex, first, last);
         } else {
             const RowView<T, false> x(xr, p.len, p.stride);
-            const int lo = min(part * p.per, p.len), hi = part + 1 == p.parts ? p.len : min(lo + p.per, p.len);
-            grad_part<T, false, kGradThreads>(x, out, lo, hi, g, c, ex, false, false);
+            const int lo = min(part * p.per, p.len);
+            GradPart<T, false, GT> g(x, lo, last ? p.len : min(lo + p.per, p.len), tid);
+            const RowGrad<T> numbers = row_grad<T, NW>(p, row, xr, tid, sm, ss, ex);
+            g.run(x, out, numbers, p.factor, ex, first, last);
         }
     }
 }
@@ -728,7 +760,8 @@ const char *const kBwd = "token_log_probs_backward";
 
 constexpr int64_t kMaxGrid = 1 << 30;
 constexpr int kRowWarps = 8;
-constexpr int kGradPart = 8192;   // elements of a block's part of a row in the gradient
+constexpr int kGradWarpRow = 2048;          // longest row of the gradient that one warp takes
+constexpr int kGradPartLeast = 4096, kGradPartMost = 32768;     // elements of a block's part of a row
 constexpr int kWarpRow = 2048;    // longest row that one warp takes
 constexpr int kWarpRowOfMany = 8192, kManyRows = 2048;
 
@@ -866,6 +899,14 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
     cudaLaunchKernelEx(&cfg, log_probs_kernel<T, VEC, ENT, kRowWarps>, p);
     h->last_kernel = p.cluster > 1 ? "log_probs_cluster" : "log_probs_block";
+}
+
+template <typename T, bool VEC, int NW> void launch_backward(Handle *h, const BackwardParams<T> &p) {
+    constexpr int kGroups = kGradThreads / (NW * 32);
+    const i128 groups = (i128)p.rows.count * p.parts;
+    const unsigned grid = (unsigned)std::min<i128>((groups + kGroups - 1) / kGroups, kMaxGrid);
+    log_probs_backward_kernel<T, VEC, NW><<<grid, kGradThreads, 0, h->stream>>>(p);
+    h->last_kernel = NW == 1 ? "log_probs_backward_warp" : "log_probs_backward_block";
 }
 
 template <typename T>
@@ -1015,21 +1056,28 @@ int backward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *token
     p.temperature = (double)temperature;
     p.inverse = 1.0 / (double)temperature;
     p.factor = exp_factor<T>(temperature);
-    p.per = kGradPart;
-    p.parts = std::max(1, (p.len + p.per - 1) / p.per);
     DeviceGuard guard(h->device);
     if (!guard.ok) return set_err(err, KX_E_NO_DEVICE, kBwd, "cannot select device");
     const bool vec = p.stride == 1 || p.len <= 1;
-    const unsigned grid = (unsigned)std::min<i128>((i128)p.rows.count * p.parts, kMaxGrid);
-    if (vec) log_probs_backward_kernel<T, true><<<grid, kGradThreads, 0, h->stream>>>(p);
-    else log_probs_backward_kernel<T, false><<<grid, kGradThreads, 0, h->stream>>>(p);
+    if (p.len <= kGradWarpRow) {
+        p.per = p.len;
+        p.parts = 1;
+        vec ? launch_backward<T, true, 1>(h, p) : launch_backward<T, false, 1>(h, p);
+    } else {
+        // even parts, as many as the device takes at once, or of the longest size
+        const int64_t wanted = std::max<int64_t>(kGradBlocks * h->sm_count / p.rows.count,
+                                                 (p.len + kGradPartMost - 1) / kGradPartMost);
+        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(wanted, p.len / kGradPartLeast));
+        p.per = ((p.len + p.parts - 1) / p.parts + 15) / 16 * 16;
+        p.parts = (p.len + p.per - 1) / p.per;
+        vec ? launch_backward<T, true, kGradThreads / 32>(h, p) : launch_backward<T, false, kGradThreads / 32>(h, p);
+    }
     const cudaError_t ce = cudaGetLastError();
     if (ce != cudaSuccess) {
         h->cuda_fail(ce);
         return cuda_err(err, h, kBwd);
     }
     ++h->launches;
-    h->last_kernel = "log_probs_backward";
     return KX_OK;
 }
 
