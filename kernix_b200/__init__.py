@@ -24,6 +24,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import operator
 import struct
 import threading
 from dataclasses import dataclass, field
@@ -537,11 +538,26 @@ class TokenLogProbs(NamedTuple):
     top_tokens: "object" = None         # [.., top], int64
 
 
-# One kx_tensor as a row of words: data, storage_len, origin, rank, then dims and
-# strides, each filled up with zeros.  These calls have many small operands
-# beside a short kernel, so their descriptors are packed, not set field by field.
-_WORDS = struct.Struct(f"={4 + MAX_RANK}Q{MAX_RANK}q")
-_PAD = [(0,) * (MAX_RANK - r) for r in range(MAX_RANK + 1)]
+# A kx_tensor of each rank as words: data, storage_len, origin, rank, then dims
+# and strides, each with zeros behind it.  These calls have many small operands
+# beside a short kernel, so descriptors are packed, not set field by field.
+_WORDS = [struct.Struct(f"={4 + r}Q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x") for r in range(MAX_RANK + 1)]
+_SIZE = C.sizeof(KxTensor)
+
+
+def _pack(buf, off: int, t) -> None:
+    """The descriptor of ``t`` at ``off`` in ``buf``."""
+    if isinstance(t, TensorView) or t.dim() > MAX_RANK:
+        C.memmove(C.addressof(buf) + off, C.byref(_descriptor(t)), _SIZE)
+        return
+    shape, stride = t.shape, t.stride()
+    rank = len(shape)
+    if t.is_contiguous():
+        _WORDS[rank].pack_into(buf, off, t.data_ptr(), t.numel(), 0, rank, *shape, *stride)
+        return
+    st = t.untyped_storage()
+    _WORDS[rank].pack_into(buf, off, st.data_ptr(), st.nbytes() // t.element_size(), t.storage_offset(), rank,
+                           *shape, *stride)
 
 
 class _Operands:
@@ -551,34 +567,19 @@ class _Operands:
 
     def __init__(self, op: str, dev: int, count: int):
         self.op, self.dev = op, dev
-        self.buf = C.create_string_buffer(_WORDS.size * count)
+        self.buf = C.create_string_buffer(_SIZE * count)
         self.at, self.used = C.addressof(self.buf), 0
-
-    def _next(self) -> int:
-        off = self.used
-        self.used = off + _WORDS.size
-        return off
 
     def add(self, name: str, t, dtype):
         if t is None:
             return None
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise InvalidParameter(f"{self.op}: {name} is {t.dtype}, not {dtype}", operation=self.op, parameter=name)
         if _device_index(t) != self.dev:
             raise InvalidParameter(f"{self.op}: {name} belongs to another device", operation=self.op, parameter=name)
-        if isinstance(t, TensorView) or len(t.shape) > MAX_RANK:
-            off = self._next()
-            C.memmove(self.at + off, C.byref(_descriptor(t)), _WORDS.size)
-            return self.at + off
-        if t.is_contiguous():
-            return self.put(t.data_ptr(), t.numel(), 0, t.shape, t.stride())
-        st = t.untyped_storage()
-        return self.put(st.data_ptr(), st.nbytes() // t.element_size(), t.storage_offset(), t.shape, t.stride())
-
-    def put(self, ptr: int, length: int, origin: int, dims, strides) -> int:
-        off, rank = self._next(), len(dims)
-        pad = _PAD[rank]
-        _WORDS.pack_into(self.buf, off, ptr, length, origin, rank, *dims, *pad, *strides, *pad)
+        off = self.used
+        self.used = off + _SIZE
+        _pack(self.buf, off, t)
         return self.at + off
 
 
@@ -605,12 +606,11 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
     dtype, device = logits.dtype, logits.device
     rows = tuple(logits.shape[:-1])
     # the numbers of each row share one allocation
-    lp, lse, ent = tokens is not None, True, bool(entropy)
-    kept = iter(torch.empty((lp + lse + ent, *rows), dtype=dtype, device=device).unbind(0))
+    kept = torch.empty((1 + (tokens is not None) + bool(entropy), *rows), dtype=dtype, device=device).unbind(0)
     out = TokenLogProbs(
-        log_probs=next(kept) if lp else None, lse=next(kept), entropy=next(kept) if ent else None,
-        top_log_probs=torch.empty((*rows, top), dtype=dtype, device=device) if top else None,
-        top_tokens=torch.empty((*rows, top), dtype=torch.int64, device=device) if top else None)
+        kept[-1] if tokens is not None else None, kept[0], kept[1] if entropy else None,
+        torch.empty((*rows, top), dtype=dtype, device=device) if top else None,
+        torch.empty((*rows, top), dtype=torch.int64, device=device) if top else None)
     token_log_probs_into(logits, tokens, out, temperature=temperature)
     return out
 
@@ -665,9 +665,7 @@ def token_log_probs_backward_into(logits, tokens, out, *, lse, entropy=None, gra
         raise_for(rc, err)
 
 
-def _one(op: str, name: str, what: str, values, allowed=1):
-    if len(values) > allowed:
-        raise InvalidParameter(f"{op}: {name} {what}", operation=op, parameter=name)
+_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
 def _lists(op: str, grads, outs=None):
@@ -678,33 +676,30 @@ def _lists(op: str, grads, outs=None):
     if not grads:
         raise InvalidParameter(f"{op}: grads (at least one)", operation=op, parameter="grads")
     lists = [("grads", grads)] if outs is None else [("grads", grads), ("outs", outs)]
-    first = grads[0]
-    flat = True
+    dtypes, devices, flat = set(), set(), True
     for name, ts in lists:
         if len(ts) != len(grads):
             raise InvalidParameter(f"{op}: {len(ts)} outs for {len(grads)} grads", operation=op, parameter=name)
-        _one(op, name, "of several dtypes", {first.dtype, *[t.dtype for t in ts]})
-        if any(isinstance(t, TensorView) for t in ts):
-            devices = {_device_index(t) for t in ts}
+        dtypes.update(map(_dtype_of, ts))
+        if TensorView in map(type, ts):
+            devices.update(map(_device_index, ts))
             flat = False
         else:
-            devices = set(map(torch.Tensor.get_device, ts))
+            devices.update(map(torch.Tensor.get_device, ts))
             flat = flat and all(map(torch.Tensor.is_contiguous, ts))
         if -1 in devices:
             raise NoDevice(f"{op}: expected CUDA tensors in {name}")
-        _one(op, name, "on several devices", {_device_index(first), *devices})
-    if outs is not None and [tuple(t.shape) for t in grads] != [tuple(t.shape) for t in outs]:
+        for what, values in (("dtypes", dtypes), ("devices", devices)):
+            if len(values) > 1:
+                raise InvalidParameter(f"{op}: {name} of several {what}", operation=op, parameter=name)
+    if outs is not None and list(map(_shape_of, grads)) != list(map(_shape_of, outs)):
         raise LayoutError(f"{op}: output shape mismatch", kind="OutputShapeMismatch")
-    if flat:
-        alone = None
-    else:
-        torch_t = [all(isinstance(t, torch.Tensor) and t.is_contiguous() for t in pair)
-                   for pair in zip(*(ts for _, ts in lists))]
-        alone = [i for i, f in enumerate(torch_t) if not f]
-    return first.dtype, [_descriptors(ts, alone) for _, ts in lists]
+    alone = () if flat else [i for i, pair in enumerate(zip(*(ts for _, ts in lists)))
+                             if not all(isinstance(t, torch.Tensor) and t.is_contiguous() for t in pair)]
+    return grads[0].dtype, [_descriptors(ts, alone) for _, ts in lists]
 
 
-def _descriptors(ts, alone=None):
+def _descriptors(ts, alone=()):
     """Descriptors of C-contiguous tensors as one axis of elements each, but for
     those at the places in ``alone``, which keep their dims and strides."""
     import torch
@@ -713,16 +708,11 @@ def _descriptors(ts, alone=None):
     every = ts if not alone else [t if isinstance(t, torch.Tensor) else t.buffer for t in ts]
     words[:, 0] = list(map(torch.Tensor.data_ptr, every))
     words[:, 4] = words[:, 1] = list(map(torch.Tensor.numel, every))     # dims[0], storage_len
-    words[:, 3] = 1                                                      # rank
-    words[:, 4 + MAX_RANK] = 1                                           # strides[0]
-    for i in alone or ():
-        t = ts[i]
-        if isinstance(t, TensorView) or len(t.shape) > MAX_RANK:
-            arr[i] = _descriptor(t)
-            continue
-        st, pad = t.untyped_storage(), _PAD[len(t.shape)]
-        _WORDS.pack_into(arr, _WORDS.size * i, st.data_ptr(), st.nbytes() // t.element_size(), t.storage_offset(),
-                         len(t.shape), *t.shape, *pad, *t.stride(), *pad)
+    words[:, 3] = words[:, 4 + MAX_RANK] = 1                             # rank, strides[0]
+    if alone:
+        words[alone] = 0
+        for i in alone:
+            _pack(arr, _SIZE * i, ts[i])
     return arr
 
 
@@ -746,7 +736,7 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     ws = torch.empty(size, dtype=torch.uint8, device=device)
     o = _Operands(op, h.device, 1)
     err = KxError()
-    tail = (o.add("norm", norm, dtype), ws.data_ptr(), size, C.byref(err))
+    tail = o.add("norm", norm, dtype), ws.data_ptr(), size, C.byref(err)
     if outs is None:
         rc = fn(h.ptr, arrays[0], n, *tail)
     else:
