@@ -603,14 +603,13 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
     if not 0 <= top <= MAX_ALTERNATIVES:
         raise InvalidParameter(f"token_log_probs: top (0 to {MAX_ALTERNATIVES} alternatives)",
                                operation="token_log_probs", parameter="top")
-    dtype, device = logits.dtype, logits.device
     rows = tuple(logits.shape[:-1])
+    empty = getattr(logits, "buffer", logits).new_empty
     # the numbers of each row share one allocation
-    kept = torch.empty((1 + (tokens is not None) + bool(entropy), *rows), dtype=dtype, device=device).unbind(0)
+    kept = empty((1 + (tokens is not None) + bool(entropy), *rows)).unbind(0)
     out = TokenLogProbs(
         kept[-1] if tokens is not None else None, kept[0], kept[1] if entropy else None,
-        torch.empty((*rows, top), dtype=dtype, device=device) if top else None,
-        torch.empty((*rows, top), dtype=torch.int64, device=device) if top else None)
+        empty((*rows, top)) if top else None, empty((*rows, top), dtype=torch.int64) if top else None)
     token_log_probs_into(logits, tokens, out, temperature=temperature)
     return out
 
@@ -641,8 +640,7 @@ def token_log_probs_backward(logits, tokens=None, *, lse, entropy=None, grad_log
     ``lse`` and (with ``grad_entropy``) ``entropy`` are the forward call's, for
     the same logits and temperature; incoming gradients have their outputs'
     dims (any strides), and one that is None counts as zero."""
-    import torch
-    out = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=logits.device)
+    out = getattr(logits, "buffer", logits).new_empty(tuple(logits.shape))
     token_log_probs_backward_into(logits, tokens, out, lse=lse, entropy=entropy, grad_log_probs=grad_log_probs,
                                   grad_entropy=grad_entropy, grad_lse=grad_lse, temperature=temperature)
     return out
@@ -728,12 +726,12 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     dtype, arrays = _lists(op, grads, outs)
     fn = _fn("kx_" + op, dtype)
     h = _bind(grads[0])
-    device = grads[0].device
+    empty = getattr(grads[0], "buffer", grads[0]).new_empty
     if norm is None:
-        norm = torch.empty((), dtype=dtype, device=device)
+        norm = empty(())
     n = len(grads)
     size = _norm_workspace(n)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    ws = empty((size,), dtype=torch.uint8)
     o = _Operands(op, h.device, 1)
     err = KxError()
     tail = o.add("norm", norm, dtype), ws.data_ptr(), size, C.byref(err)

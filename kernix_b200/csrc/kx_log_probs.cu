@@ -684,9 +684,13 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
         g.less = (T)((b - (double)g.base) * (p.inverse * unit));
     } else {
         Stats<T, false> st;
-        for (int j = tid; j < p.len; j += NW * 32) {
-            const T v[1] = {__ldg(xr + j * p.stride)};
-            st.add(v, p.factor, ex);
+        constexpr int U = 64 / (int)sizeof(T);
+        const RowView<T, false> x(xr, p.len, p.stride);
+        for (int j = tid; j < p.len; j += NW * 32 * U) {
+            T v[U][1];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x.load(j + u * NW * 32, j + u * NW * 32 < p.len, v[u]);
+            st.add(reinterpret_cast<T(&)[U]>(v), p.factor, ex);
         }
         st.template join<32>(p.factor, ex);
         if (NW > 1) {
