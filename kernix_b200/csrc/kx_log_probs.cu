@@ -242,7 +242,8 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 
 // An element as the alternatives are ordered: by value, then by place, the
 // lower one first.  For f32 both are one whole number, so that a comparison is
-// one too; the two zeros are equal.
+// one too; the two zeros are equal.  none(n) are the 512 that a row does not
+// have, behind all that it can have.
 template <typename T> struct Key;
 template <> struct Key<float> {
     uint64_t k;
@@ -252,7 +253,7 @@ template <> struct Key<float> {
         return {(uint64_t)rising << 32 | (uint32_t)~i};
     }
     __device__ static Key first() { return {~0ull}; }
-    __device__ static Key none() { return of(-INFINITY, INT_MAX); }
+    __device__ static Key none(int n) { return of(-INFINITY, INT_MAX - 512 + n); }
     __device__ bool before(const Key &o) const { return k > o.k; }
     __device__ float value() const {
         const int b = (int)((uint32_t)(k >> 32) ^ 0x80000000u);
@@ -266,7 +267,7 @@ template <> struct __align__(16) Key<double> {
     int i;
     __device__ static Key of(double v, int i) { return {v, i}; }
     __device__ static Key first() { return {(double)INFINITY, -1}; }
-    __device__ static Key none() { return {-(double)INFINITY, INT_MAX}; }
+    __device__ static Key none(int n) { return {-(double)INFINITY, INT_MAX - 512 + n}; }
     __device__ bool before(const Key &o) const { return v > o.v || (v == o.v && i < o.i); }
     __device__ double value() const { return v; }
     __device__ int place() const { return i; }
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
         }
         if (left != each) sh.slot[slots++][tid] = most;
         if (edges) {
-            const T v[1] = {lane < x.tail ? x.at(tail0 + lane) : T(-INFINITY)};
+            const T v[1] = {lane >= 16 && lane < 16 + x.tail ? x.at(tail0 + lane - 16) : T(-INFINITY)};
             st.add(v, c, ex);
         }
         const T mine = st.m;
@@ -442,14 +443,16 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
             sync();
         }
         if (p.top > 0) {
-            auto offer = [&](T v, int j) {
-                if (v >= bound && v > T(-INFINITY)) {
-                    const int k = atomicAdd(&sh.found, 1);
-                    if (k < kCandidates<NW>) sh.cand[k] = Key<T>::of(v, j);
-                }
+            auto offer = [&](int j) {
+                const int k = atomicAdd(&sh.found, 1);
+                if (k < kCandidates<NW>) sh.cand[k] = Key<T>::of(x.at(j), j);
             };
+            // Few threads have anything here, and each of them little: code
+            // that is short to fetch counts, and an offered element is read
+            // once more rather than picked out of registers.
             if (mine >= bound && st.s != T(0)) {
                 unsigned wanted = 0;
+#pragma unroll 4
                 for (int q = 0; q < slots; ++q) wanted |= (unsigned)(sh.slot[q][tid] >= bound) << q;
                 for (; wanted; wanted &= wanted - 1) {
                     const int q = __ffs(wanted) - 1;
@@ -458,19 +461,27 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
                         T v[U][VN];
 #pragma unroll
                         for (int u = 0; u < U; ++u) x.load(i + u * GT, i + u * GT < v1, v[u]);
+                        unsigned hit = 0;
 #pragma unroll
-                        for (int u = 0; u < U; ++u)
-#pragma unroll
-                            for (int k = 0; k < VN; ++k) offer(v[u][k], x.head + (i + u * GT) * VN + k);
+                        for (int k = 0; k < U * VN; ++k)
+                            hit |= (unsigned)(v[k / VN][k % VN] >= bound && v[k / VN][k % VN] > T(-INFINITY)) << k;
+                        for (; hit; hit &= hit - 1) {
+                            const int k = __ffs(hit) - 1;
+                            offer(x.head + (i + k / VN * GT) * VN + k % VN);
+                        }
                     }
                 }
-                if (edges && lane < x.head) offer(x.at(lane), lane);
-                if (edges && lane < x.tail) offer(x.at(tail0 + lane), tail0 + lane);
+                if (edges) {
+                    const int j = lane < x.head ? lane : tail0 + lane - 16;
+                    const bool there = lane < x.head || (lane >= 16 && lane < 16 + x.tail);
+                    const T v = there ? x.at(j) : T(-INFINITY);
+                    if (v >= bound && v > T(-INFINITY)) offer(j);
+                }
             }
             sync();
             const int n = sh.found;
             if (n <= kCandidates<NW>) {
-                for (int k = n + tid; k < p.top; k += GT) sh.best[k] = Key<T>::none();
+                for (int k = n + tid; k < p.top; k += GT) sh.best[k] = Key<T>::none(32 * rank + k);
                 for (int k = tid; k < n; k += GT) {
                     const Key<T> mine_k = sh.cand[k];
                     int place = 0;
@@ -481,7 +492,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
             } else {
                 Key<T> last = Key<T>::first();
                 for (int k = 0; k < p.top; ++k) {
-                    Key<T> best = Key<T>::none();
+                    Key<T> best = Key<T>::none(32 * rank + k);
                     auto look = [&](T v, int j) {
                         const Key<T> key = Key<T>::of(v, j);
                         if (last.before(key) && key.before(best)) best = key;
@@ -554,19 +565,19 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
                 int at = k;
                 if (total > p.top) {
                     // the cluster's lists, in order each: how many elements of
-                    // the others come before; what a list lacks stands behind
-                    // all that is there, in the order of the lists
-                    const int own = k / p.top;
-                    at = k % p.top;
-                    key = sh.list[own][at];
-                    for (int l = 0; l < C && at < p.top; ++l) {
-                        if (l == own) continue;
-                        for (int o = 0; o < p.top; ++o) {
-                            const Key<T> other = sh.list[l][o];
-                            if (key.before(other) || (!other.before(key) && own < l)) break;
-                            ++at;
+                    // each come before this one, by halving, in all at once
+                    key = sh.list[k / p.top][k % p.top];
+                    int less[kMaxCluster] = {};
+                    for (int by = 32; by > 0; by >>= 1) {
+#pragma unroll
+                        for (int l = 0; l < kMaxCluster; ++l) {
+                            const int to = less[l] + by;
+                            if (l < C && to <= p.top && sh.list[l][to - 1].before(key)) less[l] = to;
                         }
                     }
+                    at = 0;
+#pragma unroll
+                    for (int l = 0; l < kMaxCluster; ++l) at += less[l];
                     if (at >= p.top) continue;
                 }
                 const T v = key.value();
