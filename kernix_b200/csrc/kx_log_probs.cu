@@ -323,8 +323,12 @@ template <typename T, int NW> struct Shared {
     int found;
     Key<T> best[32];                      // the block's alternatives, in order
     Key<T> cand[kCandidates<NW>];
-    Key<T> list[NW == 1 ? 1 : kMaxCluster][32];         // the alternatives of each block of the cluster
+    Key<T> list[NW == 8 ? kMaxCluster : 1][32];         // the alternatives of each block of the cluster
 };
+
+// Blocks of one SM: 48 registers a thread for f32 (56 where a warp has a row),
+// 64 for f64 (96).
+template <typename T, int NW> constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 ? 40 : 32) / NW;
 
 // The forward pass.  One pass over the logits keeps, for each thread, the
 // maximum of its elements and the two sums against it; they meet by shuffles,
@@ -341,7 +345,7 @@ template <typename T, int NW> struct Shared {
 // ranked by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
 template <typename T, bool VEC, bool ENT, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW == 1 ? 5 : 4) : NW == 1 ? 9 : 5)
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW>)
     log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
     constexpr int kRowsPerBlock = NW == 1 ? 4 : 1;
     constexpr int GT = NW * 32;           // threads that share a row in this block
@@ -356,8 +360,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
         if (NW == 1) __syncwarp();
         else __syncthreads();
     };
-    const int C = NW == 1 ? 1 : p.cluster;
-    const int rank = NW == 1 ? 0 : blockIdx.x % C;
+    const int C = NW == 8 ? p.cluster : 1;    // only the widest blocks share a row
+    const int rank = NW == 8 ? blockIdx.x % C : 0;
     const T c = p.factor;
     const Exp<T> ex(sh.table);
     if (sizeof(T) == 8) {
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
         sync();
     }
     // the cluster's first block has to be there before the others write to it
-    if (NW > 1 && C > 1) cluster_arrive();
+    if (NW == 8 && C > 1) cluster_arrive();
     const int64_t step = (int64_t)(gridDim.x / C) * kRowsPerBlock;
     for (int64_t row = (int64_t)(blockIdx.x / C) * kRowsPerBlock + (NW == 1 ? threadIdx.x >> 5 : 0);
          row < p.rows.count; row += step) {
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
             sync();
         }
         int total = p.top;      // alternatives in best, in order
-        if (NW > 1 && C > 1) {  // one row for the cluster, which ends with it
+        if (NW == 8 && C > 1) {  // one row for the cluster, which ends with it
             cg::cluster_group cluster = cg::this_cluster();
             Shared<T, NW> *first = cluster.map_shared_rank(&sh, 0);
             cluster_wait();
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
             for (int k = tid; k < total; k += GT) {
                 Key<T> key = sh.best[k % p.top];
                 int at = k;
-                if (total > p.top) {
+                if (NW == 8 && total > p.top) {
                     // the cluster's lists, in order each: how many elements of
                     // each come before this one, by halving, in all at once
                     key = sh.list[k / p.top][k % p.top];
@@ -572,7 +576,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, sizeof(T) == 8 ? (NW 
 #pragma unroll
                         for (int l = 0; l < kMaxCluster; ++l) {
                             const int to = less[l] + by;
-                            if (l < C && to <= p.top && sh.list[l][to - 1].before(key)) less[l] = to;
+                            if (l < C && to <= p.top && sh.list[NW == 8 ? l : 0][to - 1].before(key)) less[l] = to;
                         }
                     }
                     at = 0;
@@ -774,7 +778,6 @@ const char *const kFwd = "token_log_probs";
 const char *const kBwd = "token_log_probs_backward";
 
 constexpr int64_t kMaxGrid = 1 << 30;
-constexpr int kRowWarps = 8;
 constexpr int kGradWarpRow = 2048;          // longest row of the gradient that one warp takes
 constexpr int kGradPartLeast = 4096, kGradPartMost = 32768;     // elements of a block's part of a row
 constexpr int kWarpRow = 2048;    // longest row that one warp takes
@@ -896,15 +899,27 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
         h->last_kernel = "log_probs_warp";
         return;
     }
+    // Rows that blocks of eight warps take at once have one each, or a cluster:
+    // for the SMs that would have nothing (1 x 131072 f32: 6 us in eight parts,
+    // 16 in one), or for long parts (64 x 131072: 10 us, with four parts 12).
+    // More rows than that go to blocks of four warps: twice as many rows are on
+    // their way at once while others end (4096 x 16384 with 20 alternatives:
+    // 60 us, with eight warps 67; 600 x 65536: 36 us, with eight warps 30).
+    const int64_t at_once = (int64_t)kBlocks<T, 8> * h->sm_count;
+    if (p.rows.count > at_once) {
+        log_probs_kernel<T, VEC, ENT, 4>
+            <<<(unsigned)std::min<int64_t>(p.rows.count, kMaxGrid), 128, 0, h->stream>>>(p);
+        h->last_kernel = "log_probs_block4";
+        return;
+    }
     while (p.cluster < kMaxCluster) {
         const int64_t blocks = p.rows.count * p.cluster, piece = p.len / (2 * p.cluster);
-        if (!(blocks < h->sm_count && piece >= 4096) && !(blocks < 3 * h->sm_count && piece >= 16384)) break;
+        if (!(blocks < h->sm_count && piece >= 4096) && !(2 * blocks <= at_once && piece >= 16384)) break;
         p.cluster *= 2;
     }
-    const int64_t rows = std::min<int64_t>(p.rows.count, kMaxGrid);    // all of them where there is a cluster
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * p.cluster));
-    cfg.blockDim = dim3(kRowWarps * 32);
+    cfg.gridDim = dim3((unsigned)(p.rows.count * p.cluster));
+    cfg.blockDim = dim3(256);
     cfg.stream = h->stream;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -912,8 +927,8 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    cudaLaunchKernelEx(&cfg, log_probs_kernel<T, VEC, ENT, kRowWarps>, p);
-    h->last_kernel = p.cluster > 1 ? "log_probs_cluster" : "log_probs_block";
+    cudaLaunchKernelEx(&cfg, log_probs_kernel<T, VEC, ENT, 8>, p);
+    h->last_kernel = p.cluster > 1 ? "log_probs_cluster" : "log_probs_block8";
 }
 
 template <typename T, bool VEC, int NW> void launch_backward(Handle *h, const BackwardParams<T> &p) {
