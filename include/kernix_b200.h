@@ -312,8 +312,8 @@ int kx_conv2d_backward_f64(kx_handle *h, const kx_tensor *input, const kx_tensor
  * the handle's stream, read nothing back, allocate nothing and can be captured
  * into a CUDA graph.  `tokens` and `top_tokens` hold int64 elements.
  *
- * Log probabilities of given tokens: over the last axis of `logits` (any
- * strides, 1 <= rank), with z = logits / temperature,
+ * Log probabilities of given tokens: over the last axis of `logits` (at least
+ * rank one, any strides, at most 2^30 long), with z = logits / temperature,
  *   lse       = log sum exp z,
  *   log_probs = z[token] - lse, one token for each row,
  *   entropy   = -sum p log p with p = exp(z - lse),
@@ -355,22 +355,23 @@ int kx_token_log_probs_backward_f64(kx_handle *h, const kx_tensor *logits, const
                                     const kx_tensor *lse, const kx_tensor *entropy, const kx_tensor *grad_log_probs,
                                     const kx_tensor *grad_entropy, const kx_tensor *grad_lse, double temperature,
                                     const kx_tensor *grad_logits, kx_error *err);
-/* The 2-norm over all elements of `count` gradients (0 to 2^24 of them, any
+/* The 2-norm over all elements of `count` gradients (0 to 2^20 of them, any
  * dims and strides) into the one element of `norm`, its squares added in 64
  * bits in a fixed order.  `workspace` is the caller's device memory, 8-byte
  * aligned, of at least the bytes that kx_grad_norm_workspace (host only)
  * gives; two calls that may run at the same time need one each. */
-int kx_grad_norm_workspace(uint64_t count, uint64_t *bytes);
+int kx_grad_norm_workspace(uint64_t *bytes);
 int kx_grad_norm_f32(kx_handle *h, const kx_tensor *grads, uint64_t count, const kx_tensor *norm, void *workspace,
                      uint64_t workspace_bytes, kx_error *err);
 int kx_grad_norm_f64(kx_handle *h, const kx_tensor *grads, uint64_t count, const kx_tensor *norm, void *workspace,
                      uint64_t workspace_bytes, kx_error *err);
 /* The same norm, and outs[i] = grads[i] * min(1, max_norm / norm).  Each
- * output has its gradient's dims and any strides that give each element a
- * place of its own (else KX_E_ALIAS); it may be its gradient itself (same
- * data, origin and strides), and its span overlaps no other operand
- * (KX_E_ALIAS).  With a norm of at most max_norm, or one that is not finite,
- * the outputs are the gradients as they were.  max_norm is finite and > 0. */
+ * output has its gradient's dims; its strides, in the order of their size, step
+ * over all that the smaller ones reach, so that each element has a place of its
+ * own (else KX_E_ALIAS).  It may be its gradient itself (same data, origin and
+ * strides); its span overlaps no other operand (KX_E_ALIAS).  With a norm of at
+ * most max_norm, or one that is not finite, the outputs are the gradients as
+ * they were.  max_norm is finite and > 0. */
 int kx_clip_grad_norm_f32(kx_handle *h, const kx_tensor *grads, uint64_t count, double max_norm, const kx_tensor *outs,
                           const kx_tensor *norm, void *workspace, uint64_t workspace_bytes, kx_error *err);
 int kx_clip_grad_norm_f64(kx_handle *h, const kx_tensor *grads, uint64_t count, double max_norm, const kx_tensor *outs,

@@ -24,6 +24,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import itertools
 import operator
 import struct
 import threading
@@ -674,17 +675,17 @@ def _lists(op: str, grads, outs=None):
     if not grads:
         raise InvalidParameter(f"{op}: grads (at least one)", operation=op, parameter="grads")
     lists = [("grads", grads)] if outs is None else [("grads", grads), ("outs", outs)]
-    dtypes, devices, flat = set(), set(), True
+    dtypes, devices, dense = set(), set(), []
     for name, ts in lists:
         if len(ts) != len(grads):
             raise InvalidParameter(f"{op}: {len(ts)} outs for {len(grads)} grads", operation=op, parameter=name)
         dtypes.update(map(_dtype_of, ts))
         if TensorView in map(type, ts):
             devices.update(map(_device_index, ts))
-            flat = False
+            dense.append([not isinstance(t, TensorView) and t.is_contiguous() for t in ts])
         else:
             devices.update(map(torch.Tensor.get_device, ts))
-            flat = flat and all(map(torch.Tensor.is_contiguous, ts))
+            dense.append(list(map(torch.Tensor.is_contiguous, ts)))
         if -1 in devices:
             raise NoDevice(f"{op}: expected CUDA tensors in {name}")
         for what, values in (("dtypes", dtypes), ("devices", devices)):
@@ -692,8 +693,7 @@ def _lists(op: str, grads, outs=None):
                 raise InvalidParameter(f"{op}: {name} of several {what}", operation=op, parameter=name)
     if outs is not None and list(map(_shape_of, grads)) != list(map(_shape_of, outs)):
         raise LayoutError(f"{op}: output shape mismatch", kind="OutputShapeMismatch")
-    alone = () if flat else [i for i, pair in enumerate(zip(*(ts for _, ts in lists)))
-                             if not all(isinstance(t, torch.Tensor) and t.is_contiguous() for t in pair)]
+    alone = [i for i, d in enumerate(zip(*dense)) if False in d]
     return grads[0].dtype, [_descriptors(ts, alone) for _, ts in lists]
 
 
@@ -703,21 +703,30 @@ def _descriptors(ts, alone=()):
     import torch
     arr = (KxTensor * len(ts))()
     words = np.frombuffer(arr, dtype=np.int64).reshape(len(ts), -1)
-    every = ts if not alone else [t if isinstance(t, torch.Tensor) else t.buffer for t in ts]
+    views = alone and TensorView in map(type, ts)
+    every = [t.buffer if isinstance(t, TensorView) else t for t in ts] if views else ts
     words[:, 0] = list(map(torch.Tensor.data_ptr, every))
     words[:, 4] = words[:, 1] = list(map(torch.Tensor.numel, every))     # dims[0], storage_len
     words[:, 3] = words[:, 4 + MAX_RANK] = 1                             # rank, strides[0]
-    if alone:
-        words[alone] = 0
-        for i in alone:
+    matrices = [] if views else [i for i in alone if ts[i].dim() == 2]
+    if matrices:    # transposed weights, mostly: torch's strides are not negative, so the span starts at data_ptr
+        at, rows = [ts[i] for i in matrices], np.array(matrices)
+        dims, strides = (np.fromiter(itertools.chain.from_iterable(map(f, at)), np.int64, 2 * len(at)).reshape(-1, 2)
+                         for f in (_shape_of, torch.Tensor.stride))
+        words[rows, 1] = np.where(dims.min(1) > 0, ((dims - 1) * strides).sum(1) + 1, 0)
+        words[rows, 3] = 2
+        words[rows, 4:6], words[rows, 4 + MAX_RANK:6 + MAX_RANK] = dims, strides
+    if len(matrices) < len(alone):
+        for i in sorted({*alone} - {*matrices}):
+            words[i] = 0
             _pack(arr, _SIZE * i, ts[i])
     return arr
 
 
-@functools.lru_cache(maxsize=256)
-def _norm_workspace(count: int) -> int:
+@functools.lru_cache(maxsize=1)
+def _norm_workspace() -> int:
     size = C.c_uint64()
-    raise_for(lib.kx_grad_norm_workspace(count, C.byref(size)), None)
+    raise_for(lib.kx_grad_norm_workspace(C.byref(size)), None)
     return size.value
 
 
@@ -730,7 +739,7 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     if norm is None:
         norm = empty(())
     n = len(grads)
-    size = _norm_workspace(n)
+    size = _norm_workspace()
     ws = empty((size,), dtype=torch.uint8)
     o = _Operands(op, h.device, 1)
     err = KxError()

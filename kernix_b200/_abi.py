@@ -154,7 +154,7 @@ _SIGNATURES = {
     "kx_token_log_probs_f64": (C.c_int, [*[_vp] * 3, C.c_double, *[_vp] * 5, _P(KxError)]),
     "kx_token_log_probs_backward_f32": (C.c_int, [*[_vp] * 8, C.c_float, _vp, _P(KxError)]),
     "kx_token_log_probs_backward_f64": (C.c_int, [*[_vp] * 8, C.c_double, _vp, _P(KxError)]),
-    "kx_grad_norm_workspace": (C.c_int, [_u64, _P(_u64)]),
+    "kx_grad_norm_workspace": (C.c_int, [_P(_u64)]),
     "kx_grad_norm_f32": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _u64, _P(KxError)]),
     "kx_grad_norm_f64": (C.c_int, [_vp, _vp, _u64, _vp, _vp, _u64, _P(KxError)]),
     "kx_clip_grad_norm_f32": (C.c_int, [_vp, _vp, _u64, C.c_double, _vp, _vp, _vp, _u64, _P(KxError)]),

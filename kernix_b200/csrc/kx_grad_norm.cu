@@ -173,21 +173,22 @@ __device__ __forceinline__ double add_partials(const double *partial, int64_t n)
     return block_total(s);
 }
 
-// All partial sums by one block: their root, and (total) their sum.
+// All partial sums by one block: their root, and their sum, which may take the
+// place of the first of them.
 template <typename T>
 __global__ void __launch_bounds__(1024) fold_kernel(const double *partial, int64_t n, T *norm, double *total) {
     wait_for_previous();
     const double s = add_partials(partial, n);
     if (threadIdx.x == 0) {
         *norm = (T)sqrt(s);
-        if (total) *total = s;
+        *total = s;
     }
 }
 
 template <typename T> __device__ __forceinline__ T scale_of(double sum, double max_norm, T *norm) {
     const double root = sqrt(sum);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (T)root;
-    return isfinite(root) && root > max_norm ? (T)(max_norm / root) : T(1);
+    return isfinite((T)root) && root > max_norm ? (T)(max_norm / root) : T(1);
 }
 
 // The scaled copies.  Each block adds the partial sums for itself, in one
@@ -255,14 +256,14 @@ __global__ void __launch_bounds__(kThreads) scale_strided_kernel(const T *x, T *
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr uint64_t kPartials = 2048;   // most blocks of one launch over spans,
-constexpr uint64_t kStrided = 512;     // over a tensor by itself
+constexpr int64_t kPartials = 2048;    // most blocks of one launch over spans,
+constexpr int64_t kStrided = 512;      // over a tensor by itself
+constexpr int64_t kRoom = 16384;       // partial sums that the workspace holds; then they are folded
+constexpr uint64_t kMostTensors = 1u << 20;
 constexpr int64_t kCount32 = 1ll << 31;    // 32 bits count fewer elements, and a block's step beyond them
 constexpr int64_t kFold = 2048;        // most partial sums that each block of the scaling adds
 
-uint64_t workspace_bytes(uint64_t count) {
-    return (1 + (count / kSpans + 1) * kPartials + count * kStrided) * sizeof(double);
-}
+constexpr uint64_t kWorkspace = (1 + kRoom) * sizeof(double);
 
 struct Range {
     uintptr_t a, b;
@@ -304,13 +305,13 @@ template <typename T>
 int check_lists(const kx_tensor *grads, uint64_t count, const kx_tensor *outs, const kx_tensor *norm,
                 const void *workspace, uint64_t bytes, const char *op, kx_error *err) {
     if (count && !grads) return set_err(err, KX_E_PARAM, op, "null gradients");
-    if (count > (1u << 24)) return set_err(err, KX_E_UNSUPPORTED, op, "more than 2^24 gradients");
+    if (count > kMostTensors) return set_err(err, KX_E_UNSUPPORTED, op, "more than 2^20 gradients");
     Span s;
     int rc = validate_tensor(norm, sizeof(T), &s, err);
     if (rc) return rc;
     if (numel(norm->dims, norm->rank) != 1)
         return set_err(err, KX_E_LAYOUT, op, "norm (one element)", KX_LAYOUT_OUTPUT_SHAPE_MISMATCH);
-    if (!workspace || bytes < workspace_bytes(count) || (uintptr_t)workspace % 8)
+    if (!workspace || bytes < kWorkspace || (uintptr_t)workspace % 8)
         return set_err(err, KX_E_PARAM, op, "workspace (8-byte aligned, of the size asked for)");
     std::vector<Range> all;
     all.reserve(2 * count + 2);
@@ -319,7 +320,7 @@ int check_lists(const kx_tensor *grads, uint64_t count, const kx_tensor *outs, c
             all.push_back({(uintptr_t)t->data + sp.start * sizeof(T), (uintptr_t)t->data + sp.end * sizeof(T), out});
     };
     add(norm, s, true);
-    all.push_back({(uintptr_t)workspace, (uintptr_t)workspace + workspace_bytes(count), true});
+    all.push_back({(uintptr_t)workspace, (uintptr_t)workspace + kWorkspace, true});
     uint64_t total = 0;
     for (uint64_t i = 0; i < count; ++i) {
         rc = validate_tensor(&grads[i], sizeof(T), &s, err);
@@ -407,7 +408,7 @@ bool same_strides(const kx_tensor *a, const kx_tensor *b) {
 
 unsigned blocks_for(int64_t count) {
     const int64_t b = (count + kThreads * 8 - 1) / (kThreads * 8);
-    return (unsigned)std::min<int64_t>((int64_t)kStrided, std::max<int64_t>(b, 1));
+    return (unsigned)std::min<int64_t>(kStrided, std::max<int64_t>(b, 1));
 }
 
 // One launch's worth of filled spans.
@@ -420,7 +421,7 @@ template <typename T> struct Batch {
     // clipped: 14 us, with eight blocks 16).
     unsigned blocks(const Handle *h) const {
         const unsigned some = std::min(spans.chunks, 4u * h->sm_count), more = std::min(spans.chunks / 4, 8u * h->sm_count);
-        return std::min((unsigned)kPartials, std::max(some, more));
+        return std::min<unsigned>(kPartials, std::max(some, more));
     }
 };
 
@@ -471,27 +472,33 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
         s.first[++s.n] = s.chunks;
     }
     double *total = static_cast<double *>(workspace), *partial = total + 1;
+    T *to = at<T>(norm);
     int64_t used = 0;
+    auto room = [&](int64_t blocks) {   // for that many partial sums more
+        if (used + blocks <= kRoom) return;
+        launch_after(h, fold_kernel<T>, 1, 1024, partial, used, to, partial);
+        used = 1;
+    };
     for (const Batch<T> &b : batches) {
+        room(b.blocks(h));
         sum_spans_kernel<T><<<b.blocks(h), kThreads, 0, h->stream>>>(b.spans, partial + used);
         ++h->launches;
         used += b.blocks(h);
     }
     for (uint64_t i : strided) {
         const Geom g = geom(&grads[i], nullptr);
+        const unsigned blocks = blocks_for(g.count);
+        room(blocks);
         if (g.count < kCount32)
-            sum_strided_kernel<T, uint32_t>
-                <<<blocks_for(g.count), kThreads, 0, h->stream>>>(at<T>(&grads[i]), g, partial + used);
+            sum_strided_kernel<T, uint32_t><<<blocks, kThreads, 0, h->stream>>>(at<T>(&grads[i]), g, partial + used);
         else
-            sum_strided_kernel<T, int64_t>
-                <<<blocks_for(g.count), kThreads, 0, h->stream>>>(at<T>(&grads[i]), g, partial + used);
+            sum_strided_kernel<T, int64_t><<<blocks, kThreads, 0, h->stream>>>(at<T>(&grads[i]), g, partial + used);
         ++h->launches;
-        used += blocks_for(g.count);
+        used += blocks;
     }
-    T *to = at<T>(norm);
     const double *sums = partial;
     if (!outs || used == 0 || used > kFold) {
-        launch_after(h, fold_kernel<T>, 1, 1024, partial, used, to, outs ? total : nullptr);
+        launch_after(h, fold_kernel<T>, 1, 1024, partial, used, to, total);
         sums = total;
         used = 1;
         to = nullptr;
@@ -538,9 +545,9 @@ int norm_impl(kx_handle *hh, const kx_tensor *grads, uint64_t count, double max_
 }  // namespace
 
 extern "C" {
-int kx_grad_norm_workspace(uint64_t count, uint64_t *bytes) {
-    if (!bytes || count > (1u << 24)) return KX_E_PARAM;
-    *bytes = workspace_bytes(count);
+int kx_grad_norm_workspace(uint64_t *bytes) {
+    if (!bytes) return KX_E_PARAM;
+    *bytes = kWorkspace;
     return KX_OK;
 }
 int kx_grad_norm_f32(kx_handle *h, const kx_tensor *grads, uint64_t count, const kx_tensor *norm, void *workspace,

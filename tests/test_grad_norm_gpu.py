@@ -156,6 +156,36 @@ def test_more_elements_than_32_bits_count(kx, torch_cuda):
     assert float(x.min()) == float(x.max())
 
 
+@pytest.mark.parametrize("count,rows", [(6, 1100), (45, 1100), (300, 3)])
+def test_many_tensors_with_gaps(kx, torch_cuda, count, rows):
+    """Lists whose partial sums are folded before the scaling, and on the way."""
+    torch = torch_cuda
+    shapes = [(rows, 1000)] * count
+    arrs, dev = make(torch, 23, shapes, np.float32)
+    views, hosts = [d[:, :999] for d in dev], [a[:, :999] for a in arrs]
+    check_norm(kx.grad_norm(views), hosts, np.float32)
+    before = [d[:, 999].clone() for d in dev]
+    norm = kx.clip_grad_norm_into(views, 0.25, views)
+    check_clip(norm, views, hosts, 0.25, np.float32)
+    assert all(torch.equal(d[:, 999], b) for d, b in zip(dev, before))
+
+
+def test_gaps_among_more_than_2_31_elements(kx, torch_cuda):
+    """2^31 elements of a gapped tensor, and as many places of one element."""
+    torch = torch_cuda
+    buf = torch.full((65_536, 32_769), 0.25, device="cuda")
+    view = buf[:, :32_768]
+    n = view.numel()
+    want = LD(0.25) * np.sqrt(LD(n))
+    wide = torch.full((1, 1), 0.25, device="cuda").expand(65_536, 32_768)
+    for got in (kx.grad_norm([wide]), kx.clip_grad_norm_into([view], 2.0, [view])):
+        assert abs(LD(got.item()) - want) <= want * (2.0 ** -24 + n * 2.0 ** -53)
+    by = float(LD(2.0) / want) * 0.25
+    tol = by * (3 * 2.0 ** -24 + n * 2.0 ** -53)
+    assert abs(float(view.min()) - by) <= tol and abs(float(view.max()) - by) <= tol
+    assert bool((buf[:, 32_768] == 0.25).all())
+
+
 def test_streams_graphs_and_repetition(kx, torch_cuda):
     """The same bits again, on another stream, and from two captured graphs
     that run side by side on new values."""

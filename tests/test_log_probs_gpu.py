@@ -180,6 +180,45 @@ def test_masks_ties_and_special_values(kx, torch_cuda, dtype, v):
         check_forward(run(kx, torch_cuda, x, tokens, 1.0, top), x, tokens, 1.0, dtype, top)
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("rows,v,kernel", [
+    (5, 301, "log_probs_warp"), (2100, 77, "log_probs_warp"), (2050, 2500, "log_probs_warp"),
+    (2050, 8192, "log_probs_warp"), (760, 3001, "log_probs_block4"), (150, 9001, "log_probs_block8"),
+    (200, 40001, "log_probs_cluster"), (3, 300_007, "log_probs_cluster"), (1, 1_300_001, "log_probs_cluster")])
+def test_each_kernel_and_strides(kx, torch_cuda, dtype, rows, v, kernel):
+    """Rows of every kernel, as rows and with the vocabulary's stride above one;
+    the longest make a part of a thread's elements several rounds."""
+    torch = torch_cuda
+    x, tokens = logits(13 + v, rows, v, dtype)
+    some = np.unique(np.linspace(0, rows - 1, 12).astype(int))
+    dx, dt = torch.from_numpy(x).cuda(), torch.from_numpy(tokens).cuda()
+    for view in (dx, dx.t().contiguous().t()):
+        res = kx.token_log_probs(view, dt, top=32, entropy=True)
+        assert kx.handle(0).last_kernel == kernel
+        res = numpy(kx, res, rows)
+        check_forward(kx.TokenLogProbs(*[a[some] for a in res]), x[some], tokens[some], 1.0, dtype, 32)
+        if view is dx:
+            first = res
+    # a stride changes the order of the sums alone, never the alternatives
+    assert np.array_equal(first.top_tokens, res.top_tokens)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("rows,v", [(3, 70_001), (770, 2500), (2080, 4000)])
+def test_ties_and_masks_in_each_kernel(kx, torch_cuda, dtype, rows, v):
+    """Rows of equal values, of few values, with one or no token left, most of
+    them masked, in turn."""
+    x, tokens = logits(17 + v, rows, v, dtype)
+    x[0::6] = 2.0
+    x[1::6] = np.floor(x[1::6])
+    x[2::6, 1:] = -np.inf
+    x[3::6][:, np.arange(v) % 50 != 7] = -np.inf
+    x[4::6] = -np.inf
+    some = np.unique(np.r_[0:min(rows, 12), rows - 6:rows] % rows)
+    res = run(kx, torch_cuda, x, tokens, 0.8, 20)
+    check_forward(kx.TokenLogProbs(*[a[some] for a in res]), x[some], tokens[some], 0.8, dtype, 20)
+
+
 def test_tokens_outside_the_vocabulary(kx, torch_cuda):
     x, _ = logits(8, 6, 50, np.float32)
     tokens = np.array([0, 49, -1, -100, 50, 2 ** 40], np.int64)
@@ -347,7 +386,8 @@ def backward(kx, torch, x, tokens, t, g=None, gh=None, gl=None, res=None):
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 @pytest.mark.parametrize("rows,v,t", [(1, 1, 1.0), (3, 2, 1.0), (4, 31, 0.6), (2, 130, 1.0), (5, 1000, 1.7),
-                                      (33, 1027, 1.0), (2, 4099, 1.0), (1, 32000, 0.8), (3, 50021, 1.0)])
+                                      (33, 1027, 1.0), (2, 4099, 1.0), (1, 32000, 0.8), (3, 50021, 1.0),
+                                      (1, 300_007, 1.0)])
 def test_gradient_matches_the_formula(kx, torch_cuda, dtype, rows, v, t):
     x, tokens = logits(61 + rows + v, rows, v, dtype)
     g, gh, gl = grads_in(9, rows, dtype)
