@@ -17,6 +17,8 @@
 //                                  math.rs:531-536, math_extra.rs:544-557,
 //                                  linalg_extra.rs:164-276, autograd.rs:622-690,
 //                                  neural.rs:379-430, execution.rs:149-240
+//   CudaExecutor::{token_log_probs, token_log_probs_backward, grad_norm,
+//                  clip_grad_norm}     from logits to an update (no counterpart there)
 //   kernix::shard_window / row_piece   the work split across the GPUs of a node
 //   kernix::gemm_sharded           one process over several GPUs (kx_gemm_sharded_f32)
 // Errors are exceptions carrying the C ABI's kx_error record; hooks return bool
@@ -27,6 +29,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <memory>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -68,6 +71,10 @@ template <> struct Fns<float> {
     static constexpr auto tensordot = kx_tensordot_f32;
     static constexpr auto matmul_backward = kx_matmul_backward_f32;
     static constexpr auto conv2d_backward = kx_conv2d_backward_f32;
+    static constexpr auto token_log_probs = kx_token_log_probs_f32;
+    static constexpr auto token_log_probs_backward = kx_token_log_probs_backward_f32;
+    static constexpr auto grad_norm = kx_grad_norm_f32;
+    static constexpr auto clip_grad_norm = kx_clip_grad_norm_f32;
 };
 template <> struct Fns<double> {
     static constexpr auto dense = kx_try_dense_matmul_f64;
@@ -79,6 +86,10 @@ template <> struct Fns<double> {
     static constexpr auto tensordot = kx_tensordot_f64;
     static constexpr auto matmul_backward = kx_matmul_backward_f64;
     static constexpr auto conv2d_backward = kx_conv2d_backward_f64;
+    static constexpr auto token_log_probs = kx_token_log_probs_f64;
+    static constexpr auto token_log_probs_backward = kx_token_log_probs_backward_f64;
+    static constexpr auto grad_norm = kx_grad_norm_f64;
+    static constexpr auto clip_grad_norm = kx_clip_grad_norm_f64;
 };
 }  // namespace detail
 
@@ -241,6 +252,14 @@ class DeviceTensor {
     uint64_t origin_;
 };
 
+// What token_log_probs gives for each row of logits; the alternatives only if
+// some were asked for, the entropy only if it was.
+template <typename T>
+struct TokenLogProbs {
+    std::optional<DeviceTensor<T>> log_probs, lse, entropy, top_log_probs;
+    std::optional<DeviceTensor<int64_t>> top_tokens;
+};
+
 // Device<T> + MatmulDevice<T> for one GPU.  Transfers are synchronous and in
 // physical order; matmul never changes devices or layouts behind the caller.
 class CudaExecutor {
@@ -399,8 +418,87 @@ class CudaExecutor {
         check(detail::Fns<T>::conv2d_backward(h_.get(), &dx, &dw, &dg, &opts, &dgx, &dgw, &e), e);
         return {gx, gw};
     }
+    // Log probabilities of one given token for each row of logits (its dims
+    // without the last), with the rows' log-sum-exps, the `top` (at most 32)
+    // likeliest tokens and the entropies (kx_token_log_probs_*).
+    template <typename T>
+    TokenLogProbs<T> token_log_probs(const DeviceTensor<T> &logits, const DeviceTensor<int64_t> &tokens, T temperature,
+                                     uint64_t top = 0, bool entropy = false) const {
+        std::vector<uint64_t> rows = logits.dims();
+        if (!rows.empty()) rows.pop_back();
+        TokenLogProbs<T> out;
+        out.log_probs = empty<T>(rows);
+        out.lse = empty<T>(rows);
+        if (entropy) out.entropy = empty<T>(rows);
+        if (top) {
+            rows.push_back(top);
+            out.top_log_probs = empty<T>(rows);
+            out.top_tokens = empty<int64_t>(rows);
+        }
+        kx_error e{};
+        kx_tensor dl = logits.desc(), dt = tokens.desc(), d[5];
+        check(detail::Fns<T>::token_log_probs(h_.get(), &dl, &dt, temperature, desc(out.log_probs, &d[0]),
+                                              desc(out.lse, &d[1]), desc(out.entropy, &d[2]),
+                                              desc(out.top_log_probs, &d[3]), desc(out.top_tokens, &d[4]), &e),
+              e);
+        return out;
+    }
+    // Their gradient with respect to the logits (kx_token_log_probs_backward_*);
+    // an incoming gradient that is null counts as zero.
+    template <typename T>
+    DeviceTensor<T> token_log_probs_backward(const DeviceTensor<T> &logits, const DeviceTensor<int64_t> &tokens,
+                                             const TokenLogProbs<T> &forward, T temperature,
+                                             const DeviceTensor<T> *grad_log_probs,
+                                             const DeviceTensor<T> *grad_entropy = nullptr,
+                                             const DeviceTensor<T> *grad_lse = nullptr) const {
+        auto out = empty<T>(logits.dims());
+        kx_error e{};
+        kx_tensor dl = logits.desc(), dt = tokens.desc(), dout = out.desc(), d[5];
+        auto ref = [](const DeviceTensor<T> *t, kx_tensor *to) { return t ? (*to = t->desc(), to) : nullptr; };
+        check(detail::Fns<T>::token_log_probs_backward(h_.get(), &dl, &dt, desc(forward.lse, &d[0]),
+                                                       desc(forward.entropy, &d[1]), ref(grad_log_probs, &d[2]),
+                                                       ref(grad_entropy, &d[3]), ref(grad_lse, &d[4]), temperature,
+                                                       &dout, &e),
+              e);
+        return out;
+    }
+    // The 2-norm over all elements of a list of gradients, and the list scaled
+    // in place to a norm of at most max_norm (kx_grad_norm_*, kx_clip_grad_norm_*).
+    template <typename T>
+    DeviceTensor<T> grad_norm(const std::vector<DeviceTensor<T>> &grads) const {
+        return norm_of<T>(grads, nullptr);
+    }
+    template <typename T>
+    DeviceTensor<T> clip_grad_norm(const std::vector<DeviceTensor<T>> &grads, double max_norm) const {
+        return norm_of<T>(grads, &max_norm);
+    }
 
   private:
+    template <typename T>
+    static kx_tensor *desc(const std::optional<DeviceTensor<T>> &t, kx_tensor *to) {
+        if (!t) return nullptr;
+        *to = t->desc();
+        return to;
+    }
+    template <typename T>
+    DeviceTensor<T> norm_of(const std::vector<DeviceTensor<T>> &grads, const double *max_norm) const {
+        uint64_t bytes = 0;
+        check(kx_grad_norm_workspace(&bytes), kx_error{});
+        auto norm = empty<T>({});
+        auto ws = empty<double>({(bytes + 7) / 8});
+        std::vector<kx_tensor> d;
+        for (const auto &g : grads) d.push_back(g.desc());
+        kx_error e{};
+        kx_tensor dn = norm.desc();
+        const int rc = max_norm ? detail::Fns<T>::clip_grad_norm(h_.get(), d.data(), d.size(), *max_norm, d.data(), &dn,
+                                                                 ws.buffer()->data(), bytes, &e)
+                                : detail::Fns<T>::grad_norm(h_.get(), d.data(), d.size(), &dn, ws.buffer()->data(), bytes,
+                                                            &e);
+        check(rc, e);
+        synchronize();      // the workspace ends with this call
+        return norm;
+    }
+
     Handle h_;
     int device_;
 };

@@ -96,7 +96,7 @@ class Handle:
 
     def set_stream(self, stream) -> None:
         """Order later work on ``stream`` (a torch.cuda.Stream or raw cudaStream_t)."""
-        raw = int(getattr(stream, "cuda_stream", stream) or 0)
+        raw = stream if type(stream) is int else int(getattr(stream, "cuda_stream", stream) or 0)
         if raw != self._stream:     # every call binds the current stream: skip the unchanged case
             lib.kx_set_stream(self._h, C.c_void_p(raw))
             self._stream = raw
@@ -244,7 +244,8 @@ def _current_stream(dev: int) -> int:
 
 def _bind(t) -> Handle:
     dev = _device_index(t)
-    h = getattr(_active, "handles", {}).get(dev) or handle(dev)
+    routed = getattr(_active, "handles", None)
+    h = (routed and routed.get(dev)) or _handles.get(dev) or handle(dev)
     h.set_stream(_current_stream(dev))
     return h
 
@@ -583,6 +584,14 @@ class _Operands:
         _pack(self.buf, off, t)
         return self.at + off
 
+    def fresh(self, ptr: int, count: int, dims, strides) -> int:
+        """An output that this module has just allocated, C-contiguous."""
+        off = self.used
+        self.used = off + _SIZE
+        rank = len(dims)
+        _WORDS[rank].pack_into(self.buf, off, ptr, count, 0, rank, *dims, *strides)
+        return self.at + off
+
 
 def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int = 0,
                     entropy: bool = False) -> TokenLogProbs:
@@ -600,19 +609,38 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
     NaN instead of raising: nothing is read back, so the call does not wait for
     the device and can be captured into a CUDA graph."""
     import torch
-    top = int(top)
+    op, dtype, top = "token_log_probs", logits.dtype, int(top)
     if not 0 <= top <= MAX_ALTERNATIVES:
-        raise InvalidParameter(f"token_log_probs: top (0 to {MAX_ALTERNATIVES} alternatives)",
-                               operation="token_log_probs", parameter="top")
-    rows = tuple(logits.shape[:-1])
+        raise InvalidParameter(f"{op}: top (0 to {MAX_ALTERNATIVES} alternatives)", operation=op, parameter="top")
+    fn = _fn("kx_token_log_probs", dtype)
+    h = _bind(logits)
+    o = _Operands(op, h.device, 7)
+    given = o.add("logits", logits, dtype), o.add("tokens", tokens, torch.int64)
     empty = getattr(logits, "buffer", logits).new_empty
-    # the numbers of each row share one allocation
-    kept = empty((1 + (tokens is not None) + bool(entropy), *rows)).unbind(0)
-    out = TokenLogProbs(
-        kept[-1] if tokens is not None else None, kept[0], kept[1] if entropy else None,
-        empty((*rows, top)) if top else None, empty((*rows, top), dtype=torch.int64) if top else None)
-    token_log_probs_into(logits, tokens, out, temperature=temperature)
-    return out
+    # the numbers of each row share one allocation: [lse, entropy, log_probs]
+    rows = tuple(logits.shape[:-1])
+    n = 1 + bool(entropy) + (tokens is not None)
+    kept = empty((n, *rows))
+    at, strides = kept.data_ptr(), kept.stride()[1:]
+    count = kept.numel() // n
+    size = count * kept.element_size()
+    lse, lp, ent, top_lp, top_ids = o.fresh(at, count, rows, strides), None, None, None, None
+    if entropy:
+        ent = o.fresh(at + size, count, rows, strides)
+    if tokens is not None:
+        lp = o.fresh(at + (n - 1) * size, count, rows, strides)
+    values = ids = None
+    if top:
+        values, ids = empty((*rows, top)), empty((*rows, top), dtype=torch.int64)
+        dims, strides = values.shape, values.stride()
+        top_lp = o.fresh(values.data_ptr(), count * top, dims, strides)
+        top_ids = o.fresh(ids.data_ptr(), count * top, dims, strides)
+    err = KxError()
+    rc = fn(h.ptr, *given, float(temperature), lp, lse, ent, top_lp, top_ids, C.byref(err))
+    if rc:
+        raise_for(rc, err)
+    kept = kept.unbind(0)
+    return TokenLogProbs(kept[-1] if tokens is not None else None, kept[0], kept[1] if entropy else None, values, ids)
 
 
 def token_log_probs_into(logits, tokens, out: TokenLogProbs, *, temperature: float = 1.0) -> None:
@@ -693,7 +721,7 @@ def _lists(op: str, grads, outs=None):
                 raise InvalidParameter(f"{op}: {name} of several {what}", operation=op, parameter=name)
     if outs is not None and list(map(_shape_of, grads)) != list(map(_shape_of, outs)):
         raise LayoutError(f"{op}: output shape mismatch", kind="OutputShapeMismatch")
-    alone = [i for i, d in enumerate(zip(*dense)) if False in d]
+    alone = [i for i, d in enumerate(zip(*dense)) if False in d] if any(False in d for d in dense) else ()
     return grads[0].dtype, [_descriptors(ts, alone) for _, ts in lists]
 
 
