@@ -300,7 +300,9 @@ template <typename T> __device__ __forceinline__ T falling_again(T v, int lane) 
     return v;
 }
 
-// The q-th largest of the warp's lane values.
+// The q-th largest of the warp's lane values.  Up to six are found one by one,
+// in blocks of four and eight warps (2500 x 30000 f32 with 8 alternatives: 57.4
+// us, sorting always 58.4).
 template <typename T> __device__ __forceinline__ T largest(T v, int q, int lane) {
     if (q > 6) return __shfl_sync(0xffffffffu, sorted_falling(v, lane), q - 1);
     for (; q > 1; --q) {
@@ -312,7 +314,10 @@ template <typename T> __device__ __forceinline__ T largest(T v, int q, int lane)
 
 template <int NW> constexpr int kCandidates = NW == 1 ? 256 : 512;
 constexpr int kMaxCluster = 8;
-constexpr int kWarpTop = 12;      // alternatives for which one warp's 32 maxima bound well
+// Alternatives for which one warp's 32 maxima bound well: beyond them the bound
+// comes from the maxima of the parts (4096 x 1000 f32 with 32 alternatives:
+// 13 us, with the 32 maxima 46; with 16 alternatives 11.7 and 10.5).
+constexpr int kWarpTop = 20;
 template <int NW> constexpr int kSlots = NW == 1 ? 8 : 16;
 
 template <typename T, int NW> struct Shared {
@@ -334,15 +339,19 @@ template <typename T, int NW> constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 
 // maximum of its elements and the two sums against it; they meet by shuffles,
 // then in shared memory, then (few rows) in that of the cluster's first block,
 // so that one launch and no workspace do for any number of rows.  The bound is
-// the reading of the logits; the instructions for an element are about eight.
+// the reading of the logits: 4096 x 32000 f32 with entropies takes 85 us, 6.1
+// TB/s; in f64 it is the 64-bit pipe, 46 % busy over the 53 us of 509 x 32003,
+// where more registers would be needed to keep it fed.  Few rows wait for one
+// memory round trip after another: 1 x 32000 f32 takes 5.8 us, with
+// alternatives 8 to 9.
 //
 // The alternatives come from the threads' maxima: the K-th largest of them, or
 // less, bounds the K-th alternative from below, so only elements at or above
 // it matter.  Threads whose maximum reaches it (a few times K) read the parts
-// of theirs again whose own maxima do, which is one round trip to memory at
-// about 1 % of the row: going over all of their elements took 97 us where this
-// takes %FIG% (1501 x 50021 f32, 8 alternatives).  A few dozen candidates are
-// ranked by counting.  Should more than kCandidates elements reach the bound (rows of
+// of theirs again whose own maxima do, about 5 % of the row: going over all of
+// their elements took 97 us where this takes 72 (1501 x 50021 f32, 8
+// alternatives, half of the tokens masked).  A few dozen candidates are ranked
+// by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
 template <typename T, bool VEC, bool ENT, int NW>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW>)
@@ -732,11 +741,14 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
 }
 
 // The gradient: one element in, one out, with a row's few numbers between
-// them.  The bound is the two streams.  A block takes a part of one row (long
-// parts where there are many rows: 4096 x 32000 f32 in parts of %G1%), or each
-// of its warps a short row.
+// them.  The bound is the two streams: 4096 x 32000 f32 takes 166 us, 6.3
+// TB/s.  A block takes a part of one row: parts of 32000 elements there, where
+// parts of 8192 took 190 us and of 2048 343, as each begins with its row's
+// numbers; or each of its warps a short row (4096 x 1000: 8 us, with a block
+// for each row 23).
 template <typename T, bool VEC, int NW>
-__global__ void __launch_bounds__(kGradThreads, kGradBlocks) log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
+__global__ void __launch_bounds__(kGradThreads, kGradBlocks)
+    log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
     constexpr int GT = NW * 32;
     constexpr int kGroups = kGradThreads / GT;
     __shared__ T sm[NW], ss[NW];
@@ -778,11 +790,20 @@ const char *const kFwd = "token_log_probs";
 const char *const kBwd = "token_log_probs_backward";
 
 constexpr int64_t kMaxGrid = 1 << 30;
-constexpr int kGradWarpRow = 2048;          // longest row of the gradient that one warp takes
-constexpr int kGradPartLeast = 4096, kGradPartMost = 32768;     // elements of a block's part of a row
-constexpr int kWarpRow = 2048;    // longest row that one warp takes
-constexpr int kWarpRowOfMany = 8192, kManyRows = 2048;
-
+// Longest row that one warp takes: where there are more rows than blocks of
+// eight warps at once 16 KB (4096 x 2048 f32 with 8 alternatives: 12 us, with a
+// block for each row 19; 4096 x 8192 with 20: 38 and 37; 1000 x 2048 f64 12 and
+// 12), else what gives each thread of such a block less than 16 bytes (64 x
+// 2000 f32 with 8 alternatives: 8.2 us, in blocks 6.2).
+constexpr int kWarpRowBytes = 16384, kWarpRow = 1024;
+// Longest row of the gradient that one warp takes: 4096 x 2000 f32 13 us, in
+// blocks 27; 4096 x 4096 29 us, in blocks 27.
+constexpr int kGradWarpRow = 2048;
+// Elements of a block's part of a row in the gradient: no fewer, for the few
+// rows that are cut for the SMs' sake (8 x 30208 f32: 5.5 us, in parts of 16384
+// 7.5), and no more, for the last blocks to end together (1501 x 50021: 103 us,
+// whole rows 108).
+constexpr int kGradPartLeast = 4096, kGradPartMost = 32768;
 // The temperature divides logits: it and its reciprocal are normal numbers.
 template <typename T> bool temperature_ok(T t) {
     return std::isnormal((double)t) && t > T(0) && std::isnormal(exp_factor<T>(t));
@@ -893,7 +914,9 @@ int row_output(const kx_tensor *t, const kx_tensor *logits, uint32_t es, const c
 
 template <typename T, bool VEC, bool ENT>
 void launch_forward(Handle *h, ForwardParams<T> &p) {
-    if (p.len <= kWarpRow || (p.len <= kWarpRowOfMany && p.rows.count >= kManyRows)) {
+    const int64_t at_once = (int64_t)kBlocks<T, 8> * h->sm_count;
+    const bool many = p.rows.count > at_once;
+    if (p.len <= (many ? kWarpRowBytes / (int)sizeof(T) : kWarpRow)) {
         const int64_t blocks = (p.rows.count + 3) / 4;
         log_probs_kernel<T, VEC, ENT, 1><<<(unsigned)std::min<int64_t>(blocks, kMaxGrid), 128, 0, h->stream>>>(p);
         h->last_kernel = "log_probs_warp";
@@ -905,8 +928,7 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     // More rows than that go to blocks of four warps: twice as many rows are on
     // their way at once while others end (4096 x 16384 with 20 alternatives:
     // 60 us, with eight warps 67; 600 x 65536: 36 us, with eight warps 30).
-    const int64_t at_once = (int64_t)kBlocks<T, 8> * h->sm_count;
-    if (p.rows.count > at_once) {
+    if (many) {
         log_probs_kernel<T, VEC, ENT, 4>
             <<<(unsigned)std::min<int64_t>(p.rows.count, kMaxGrid), 128, 0, h->stream>>>(p);
         h->last_kernel = "log_probs_block4";

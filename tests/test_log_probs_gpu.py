@@ -182,9 +182,9 @@ def test_masks_ties_and_special_values(kx, torch_cuda, dtype, v):
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 @pytest.mark.parametrize("rows,v,kernel", [
-    (5, 301, "log_probs_warp"), (2100, 77, "log_probs_warp"), (2050, 2500, "log_probs_warp"),
-    (2050, 8192, "log_probs_warp"), (760, 3001, "log_probs_block4"), (150, 9001, "log_probs_block8"),
-    (200, 40001, "log_probs_cluster"), (3, 300_007, "log_probs_cluster"), (1, 1_300_001, "log_probs_cluster")])
+    (5, 301, "log_probs_warp"), (2100, 77, "log_probs_warp"), (760, 1501, "log_probs_warp"),
+    (2050, 2048, "log_probs_warp"), (760, 5001, "log_probs_block4"), (150, 9001, "log_probs_block8"),
+    (40, 1025, "log_probs_block8"), (200, 40001, "log_probs_cluster"), (3, 300_007, "log_probs_cluster"), (1, 1_300_001, "log_probs_cluster")])
 def test_each_kernel_and_strides(kx, torch_cuda, dtype, rows, v, kernel):
     """Rows of every kernel, as rows and with the vocabulary's stride above one;
     the longest make a part of a thread's elements several rounds."""
@@ -204,7 +204,7 @@ def test_each_kernel_and_strides(kx, torch_cuda, dtype, rows, v, kernel):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
-@pytest.mark.parametrize("rows,v", [(3, 70_001), (770, 2500), (2080, 4000)])
+@pytest.mark.parametrize("rows,v", [(3, 70_001), (770, 4500), (2080, 2000), (64, 1500)])
 def test_ties_and_masks_in_each_kernel(kx, torch_cuda, dtype, rows, v):
     """Rows of equal values, of few values, with one or no token left, most of
     them masked, in turn."""
