@@ -69,6 +69,7 @@ class Handle:
         raise_for(lib.kx_create(device, C.byref(ptr), C.byref(err)), err)
         self._h = ptr
         self._stream = 0            # the raw stream the library handle orders work on
+        self._turn = threading.Lock()
 
     @classmethod
     def adopt(cls, ptr: C.c_void_p, device: int) -> "Handle":
@@ -77,6 +78,7 @@ class Handle:
         h.device = device
         h._h = ptr
         h._stream = 0
+        h._turn = threading.Lock()
         return h
 
     @property
@@ -242,11 +244,15 @@ def _current_stream(dev: int) -> int:
     return int(raw(dev)) if raw is not None else int(torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _bind(t) -> Handle:
+def _route(t) -> Handle:
     dev = _device_index(t)
     routed = getattr(_active, "handles", None)
-    h = (routed and routed.get(dev)) or _handles.get(dev) or handle(dev)
-    h.set_stream(_current_stream(dev))
+    return (routed and routed.get(dev)) or _handles.get(dev) or handle(dev)
+
+
+def _bind(t) -> Handle:
+    h = _route(t)
+    h.set_stream(_current_stream(h.device))
     return h
 
 
@@ -540,6 +546,17 @@ class TokenLogProbs(NamedTuple):
     top_tokens: "object" = None         # [.., top], int64
 
 
+def _enqueue(h: Handle, fn, *args) -> None:
+    """The library call ``fn`` on the current stream, in one turn: threads that
+    share a handle must not change its stream between the two."""
+    err = KxError()
+    with h._turn:
+        h.set_stream(_current_stream(h.device))
+        rc = fn(h._h, *args, C.byref(err))
+    if rc:
+        raise_for(rc, err)
+
+
 # A kx_tensor of each rank as words: data, storage_len, origin, rank, then dims
 # and strides, each with zeros behind it.  These calls have many small operands
 # beside a short kernel, so descriptors are packed, not set field by field.
@@ -613,7 +630,7 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
     if not 0 <= top <= MAX_ALTERNATIVES:
         raise InvalidParameter(f"{op}: top (0 to {MAX_ALTERNATIVES} alternatives)", operation=op, parameter="top")
     fn = _fn("kx_token_log_probs", dtype)
-    h = _bind(logits)
+    h = _route(logits)
     o = _Operands(op, h.device, 7)
     given = o.add("logits", logits, dtype), o.add("tokens", tokens, torch.int64)
     empty = getattr(logits, "buffer", logits).new_empty
@@ -635,10 +652,7 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
         dims, strides = values.shape, values.stride()
         top_lp = o.fresh(values.data_ptr(), count * top, dims, strides)
         top_ids = o.fresh(ids.data_ptr(), count * top, dims, strides)
-    err = KxError()
-    rc = fn(h.ptr, *given, float(temperature), lp, lse, ent, top_lp, top_ids, C.byref(err))
-    if rc:
-        raise_for(rc, err)
+    _enqueue(h, fn, *given, float(temperature), lp, lse, ent, top_lp, top_ids)
     kept = kept.unbind(0)
     return TokenLogProbs(kept[-1] if tokens is not None else None, kept[0], kept[1] if entropy else None, values, ids)
 
@@ -649,15 +663,12 @@ def token_log_probs_into(logits, tokens, out: TokenLogProbs, *, temperature: flo
     import torch
     dtype, int64 = logits.dtype, torch.int64
     fn = _fn("kx_token_log_probs", dtype)
-    h = _bind(logits)
+    h = _route(logits)
     o = _Operands("token_log_probs", h.device, 7)
-    err = KxError()
-    rc = fn(h.ptr, o.add("logits", logits, dtype), o.add("tokens", tokens, int64), float(temperature),
-            o.add("log_probs", out.log_probs, dtype), o.add("lse", out.lse, dtype),
-            o.add("entropy", out.entropy, dtype), o.add("top_log_probs", out.top_log_probs, dtype),
-            o.add("top_tokens", out.top_tokens, int64), C.byref(err))
-    if rc:
-        raise_for(rc, err)
+    _enqueue(h, fn, o.add("logits", logits, dtype), o.add("tokens", tokens, int64), float(temperature),
+             o.add("log_probs", out.log_probs, dtype), o.add("lse", out.lse, dtype),
+             o.add("entropy", out.entropy, dtype), o.add("top_log_probs", out.top_log_probs, dtype),
+             o.add("top_tokens", out.top_tokens, int64))
 
 
 def token_log_probs_backward(logits, tokens=None, *, lse, entropy=None, grad_log_probs=None, grad_entropy=None,
@@ -681,15 +692,12 @@ def token_log_probs_backward_into(logits, tokens, out, *, lse, entropy=None, gra
     import torch
     dtype = logits.dtype
     fn = _fn("kx_token_log_probs_backward", dtype)
-    h = _bind(logits)
+    h = _route(logits)
     o = _Operands("token_log_probs_backward", h.device, 8)
-    err = KxError()
-    rc = fn(h.ptr, o.add("logits", logits, dtype), o.add("tokens", tokens, torch.int64), o.add("lse", lse, dtype),
-            o.add("entropy", entropy, dtype), o.add("grad_log_probs", grad_log_probs, dtype),
-            o.add("grad_entropy", grad_entropy, dtype), o.add("grad_lse", grad_lse, dtype), float(temperature),
-            o.add("out", out, dtype), C.byref(err))
-    if rc:
-        raise_for(rc, err)
+    _enqueue(h, fn, o.add("logits", logits, dtype), o.add("tokens", tokens, torch.int64), o.add("lse", lse, dtype),
+             o.add("entropy", entropy, dtype), o.add("grad_log_probs", grad_log_probs, dtype),
+             o.add("grad_entropy", grad_entropy, dtype), o.add("grad_lse", grad_lse, dtype), float(temperature),
+             o.add("out", out, dtype))
 
 
 _dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
@@ -762,7 +770,7 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     import torch
     dtype, arrays = _lists(op, grads, outs)
     fn = _fn("kx_" + op, dtype)
-    h = _bind(grads[0])
+    h = _route(grads[0])
     empty = getattr(grads[0], "buffer", grads[0]).new_empty
     if norm is None:
         norm = empty(())
@@ -770,14 +778,11 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     size = _norm_workspace()
     ws = empty((size,), dtype=torch.uint8)
     o = _Operands(op, h.device, 1)
-    err = KxError()
-    tail = o.add("norm", norm, dtype), ws.data_ptr(), size, C.byref(err)
+    tail = o.add("norm", norm, dtype), ws.data_ptr(), size
     if outs is None:
-        rc = fn(h.ptr, arrays[0], n, *tail)
+        _enqueue(h, fn, arrays[0], n, *tail)
     else:
-        rc = fn(h.ptr, arrays[0], n, float(max_norm), arrays[1], *tail)
-    if rc:
-        raise_for(rc, err)
+        _enqueue(h, fn, arrays[0], n, float(max_norm), arrays[1], *tail)
     return norm
 
 

@@ -305,3 +305,36 @@ def test_a_serving_step(kx, torch_cuda):
     lp = kx.token_log_probs(z, tokens, temperature=0.8).log_probs
     assert torch.equal(lp, out.top_log_probs.gather(1, pick)[:, 0])
     assert torch.equal(out.top_tokens[:, 0], z.argmax(-1))
+
+
+def test_calls_of_several_threads(kx, torch_cuda):
+    """Threads that share the default handle, each on a stream of its own: what
+    each one enqueues runs in its own order."""
+    import threading
+
+    torch = torch_cuda
+    x0, tokens = torch.randn(40, 3001, device="cuda"), torch.arange(40, device="cuda")
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(60):
+                x = x0 * (1 + 0.01 * k) + 0.001 * i     # written on this stream right before it is read
+                out = kx.token_log_probs(x, tokens, top=3)
+                grad = kx.token_log_probs_backward(x, tokens, lse=out.lse, grad_log_probs=out.lse)
+                norm, (clipped,) = kx.clip_grad_norm([grad], 0.5)
+                lse = torch.logsumexp(x, -1)
+                # sums of 3001 terms in f32: 3001 2^-24 at the very most, of about 8
+                if not bool(((out.lse - lse).abs() <= 4e-4 * lse.abs()).all()) or not torch.equal(
+                        out.top_tokens[:, 0], x.argmax(-1)):
+                    wrong.append((k, i))
+                if abs(float(torch.linalg.vector_norm(clipped)) - 0.5) > 1e-3 or float(norm) <= 0.5:
+                    wrong.append((k, i, "norm"))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

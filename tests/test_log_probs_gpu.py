@@ -263,6 +263,27 @@ def test_layouts(kx, torch_cuda, dtype, v):
           tokens.reshape(2, 3).T.reshape(-1), dt.reshape(2, 3).t())
 
 
+def test_most_axes_and_another_handle(kx, torch_cuda):
+    """Eight axes of which few nest, through a handle of the caller's own."""
+    torch = torch_cuda
+    x, tokens = logits(33, 24, 130, np.float32)
+    shape = (2, 1, 3, 1, 2, 1, 2, 130)
+    dx = torch.from_numpy(x).cuda().reshape(shape)
+    dt = torch.from_numpy(tokens).cuda().reshape(shape[:-1])
+    order = (2, 1, 6, 3, 0, 5, 4)
+    rows = np.arange(24).reshape(shape[:-1]).transpose(order).reshape(-1)
+    own = kx.Handle(0)
+    with kx.using(own):
+        res = kx.token_log_probs(dx.permute(*order, 7), dt.permute(order), top=3, entropy=True)
+    assert own.launches == 1 and res.top_tokens.shape == tuple(shape[i] for i in order) + (3,)
+    check_forward(numpy(kx, res, 24), x[rows], tokens[rows], 1.0, np.float32, 3)
+    g = torch.ones(shape[:-1], device="cuda").permute(order)
+    got = kx.token_log_probs_backward(dx.permute(*order, 7), dt.permute(order), lse=res.lse, grad_log_probs=g)
+    check_backward(got.cpu().numpy().reshape(24, 130), x[rows], tokens[rows], 1.0, np.float32, np.ones(24, np.float32))
+    own.synchronize()
+    own.close()
+
+
 def test_shapes_without_rows_or_vocabulary(kx, torch_cuda):
     torch = torch_cuda
     res = kx.token_log_probs(torch.zeros(0, 5, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), top=2)
