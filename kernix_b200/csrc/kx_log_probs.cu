@@ -623,6 +623,7 @@ constexpr double kLseTrusted = 256.0;
 //   dx = p (a - b l)  [+ at the token]
 template <typename T> struct RowGrad {
     T base, less, a, b, at_token;
+    T nothing;      // of an element whose probability is 0: NaN where the row's numbers are
     int token;
     __device__ __forceinline__ T operator()(T v, T c, const Exp<T> &ex) const {
         const T l = fma(v - base, c, -less);
@@ -630,7 +631,8 @@ template <typename T> struct RowGrad {
             const T d = ex(l) * fma(-b, larger(l, T(-1e5)), a);
             return v == T(-INFINITY) ? T(0) : d;
         } else {
-            return Exp<T>::counts(l) ? ex(l) * fma(-b, l, a) : T(0);
+            if (Exp<T>::counts(l)) return ex(l) * fma(-b, l, a);
+            return v == T(-INFINITY) ? T(0) : nothing;
         }
     }
 };
@@ -736,6 +738,7 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
     g.a = (T)((double)(gl - gp - gh * h) * p.inverse);
     g.b = (T)((double)gh * (p.inverse / unit));
     g.at_token = (T)((double)gp * p.inverse);
+    g.nothing = g.a * T(0);
     g.token = t >= 0 && t < p.len ? (int)t : -1;
     return g;
 }

@@ -439,6 +439,19 @@ def test_gradient_of_masks_and_special_values(kx, torch_cuda, dtype, v):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_gradient_of_an_impossible_token_is_nan_everywhere(kx, torch_cuda, dtype):
+    """Where probabilities are 0 too, but for masked logits."""
+    x, _ = logits(77, 3, 700, dtype)
+    x[:, 1::2] -= 3000
+    x[:, 5] = -np.inf
+    tokens = np.array([700, 0, 10 ** 12], np.int64)
+    got = backward(kx, torch_cuda, x, tokens, 1.0, np.ones(3, dtype))
+    for r in (0, 2):
+        assert got[r, 5] == 0 and np.isnan(np.delete(got[r], 5)).all()
+    check_backward(got[1:2], x[1:2], tokens[1:2], 1.0, dtype, np.ones(1, dtype))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
 @pytest.mark.parametrize("v", [9, 1100, 5001])
 def test_gradient_layouts(kx, torch_cuda, dtype, v):
     """Logits at every alignment against the gradient's, a vocabulary of
