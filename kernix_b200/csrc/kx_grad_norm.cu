@@ -3,8 +3,8 @@
 //
 //   norm = sqrt(sum over all tensors of g^2),  out = g * min(1, max_norm / norm)
 //
-// Squares are added in 64 bits in an order that only the sizes and the device
-// fix, so the same gradients give the same bits again.  A norm that is not
+// Squares are added in 64 bits in an order that only the gradients' sizes and
+// strides and the device fix, so the same gradients give the same bits again.  A norm that is not
 // finite scales nothing: the outputs are the gradients as they were.
 #include <algorithm>
 #include <cmath>
@@ -85,13 +85,13 @@ __device__ __forceinline__ void offsets(const Geom &g, I i, int64_t &so, int64_t
 
 // The same total in each thread of the block, of which this is the one call.
 __device__ double block_total(double v) {
-    __shared__ double red[32];
-    const int warps = blockDim.x >> 5;
+    constexpr int kWarps = kThreads / 32;
+    __shared__ double red[kWarps];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    double s = (int)(threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.0;
+    double s = (threadIdx.x & 31) < kWarps ? red[threadIdx.x & 31] : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
@@ -169,14 +169,14 @@ __global__ void __launch_bounds__(kThreads) sum_strided_kernel(const T *__restri
 
 __device__ __forceinline__ double add_partials(const double *partial, int64_t n) {
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += partial[i];
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) s += partial[i];
     return block_total(s);
 }
 
-// All partial sums by one block: their root, and their sum, which may take the
-// place of the first of them.
+// All partial sums by one block, in the order in which each block of the scaling
+// adds them: their root, and their sum, which may take the place of the first.
 template <typename T>
-__global__ void __launch_bounds__(1024) fold_kernel(const double *partial, int64_t n, T *norm, double *total) {
+__global__ void __launch_bounds__(kThreads) fold_kernel(const double *partial, int64_t n, T *norm, double *total) {
     wait_for_previous();
     const double s = add_partials(partial, n);
     if (threadIdx.x == 0) {
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) scale_spans_kernel(const __grid_cons
         while (c < g.first[k]) --k;
         const T *x = g.src[k];
         T *y = out.dst[k];
-        if (by == T(1) && x == y) continue;
+        if (!y || (by == T(1) && x == y)) continue;     // scaled by itself, or in place already
         const Cut<T> cut(x, g.len[k]);
         const uint32_t part = c - g.first[k];
         if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0) {
@@ -429,10 +429,10 @@ template <typename T> struct Batch {
 // A kernel that may start while the previous one ends; it waits by itself for
 // that one's results (griddepcontrol.wait).
 template <typename... Params, typename... Args>
-void launch_after(Handle *h, void (*kernel)(Params...), unsigned blocks, unsigned threads, Args... args) {
+void launch_after(Handle *h, void (*kernel)(Params...), unsigned blocks, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = dim3(kThreads);
     cfg.stream = h->stream;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -446,14 +446,18 @@ void launch_after(Handle *h, void (*kernel)(Params...), unsigned blocks, unsigne
 template <typename T>
 int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_norm, const kx_tensor *outs,
                const kx_tensor *norm, void *workspace, const char *op, kx_error *err) {
-    // which tensors are runs of memory; the rest go one by one
+    // which tensors are runs of memory; the rest go one by one, and so does the
+    // scaling into an output of other strides, so that the sums are the same
+    // whatever the outputs are
     std::vector<Batch<T>> batches;
-    std::vector<uint64_t> strided;
+    std::vector<uint64_t> strided, apart;
     for (uint64_t i = 0; i < count; ++i) {
         const int64_t n = (int64_t)numel(grads[i].dims, grads[i].rank);
         if (n == 0) continue;
         const int64_t low = filled_span(&grads[i]);
-        if (low > 0 || (outs && !same_strides(&grads[i], &outs[i]))) {
+        const bool alike = outs && same_strides(&grads[i], &outs[i]);
+        if (outs && (low > 0 || !alike)) apart.push_back(i);
+        if (low > 0) {
             strided.push_back(i);
             continue;
         }
@@ -468,7 +472,7 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
         s.src[s.n] = at<T>(&grads[i]) + low;
         s.len[s.n] = n;
         s.first[s.n] = s.chunks;
-        batches.back().outs.dst[s.n] = outs ? at<T>(&outs[i]) + low : nullptr;
+        batches.back().outs.dst[s.n] = alike ? at<T>(&outs[i]) + low : nullptr;
         s.chunks += chunks;
         s.first[++s.n] = s.chunks;
     }
@@ -477,7 +481,7 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
     int64_t used = 0;
     auto room = [&](int64_t blocks) {   // for that many partial sums more
         if (used + blocks <= kRoom) return;
-        launch_after(h, fold_kernel<T>, 1, 1024, partial, used, to, partial);
+        launch_after(h, fold_kernel<T>, 1, partial, used, to, partial);
         used = 1;
     };
     for (const Batch<T> &b : batches) {
@@ -499,20 +503,20 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
     }
     const double *sums = partial;
     if (!outs || used == 0 || used > kFold) {
-        launch_after(h, fold_kernel<T>, 1, 1024, partial, used, to, total);
+        launch_after(h, fold_kernel<T>, 1, partial, used, to, total);
         sums = total;
         used = 1;
         to = nullptr;
     }
     if (outs) {
         for (const Batch<T> &b : batches) {
-            launch_after(h, scale_spans_kernel<T>, b.blocks(h), kThreads, b.spans, b.outs, sums, used, max_norm, to);
+            launch_after(h, scale_spans_kernel<T>, b.blocks(h), b.spans, b.outs, sums, used, max_norm, to);
             to = nullptr;
         }
-        for (uint64_t i : strided) {
+        for (uint64_t i : apart) {
             const Geom g = geom(&grads[i], &outs[i]);
             launch_after(h, g.count < kCount32 ? scale_strided_kernel<T, uint32_t> : scale_strided_kernel<T, int64_t>,
-                         blocks_for(g.count), kThreads, at<T>(&grads[i]), at<T>(&outs[i]), g, sums, used, max_norm, to);
+                         blocks_for(g.count), at<T>(&grads[i]), at<T>(&outs[i]), g, sums, used, max_norm, to);
             to = nullptr;
         }
     }

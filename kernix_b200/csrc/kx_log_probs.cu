@@ -331,9 +331,10 @@ template <typename T, int NW> struct Shared {
     Key<T> list[NW == 8 ? kMaxCluster : 1][32];         // the alternatives of each block of the cluster
 };
 
-// Blocks of one SM: 48 registers a thread for f32 (56 where a warp has a row),
-// 64 for f64 (96).
-template <typename T, int NW> constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 ? 40 : 32) / NW;
+// Blocks of one SM: 48 registers a thread for f32 (56 where a warp has a row,
+// 64 with WIDE, which has twice the loads in flight), 64 for f64 (96).
+template <typename T, int NW, bool WIDE>
+constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 && !WIDE ? 40 : 32) / NW;
 
 // The forward pass.  One pass over the logits keeps, for each thread, the
 // maximum of its elements and the two sums against it; they meet by shuffles,
@@ -353,13 +354,13 @@ template <typename T, int NW> constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 
 // alternatives, half of the tokens masked).  A few dozen candidates are ranked
 // by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
-template <typename T, bool VEC, bool ENT, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW>)
+template <typename T, bool VEC, bool ENT, int NW, bool WIDE = false>
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
     log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
     constexpr int kRowsPerBlock = NW == 1 ? 4 : 1;
     constexpr int GT = NW * 32;           // threads that share a row in this block
     constexpr int VN = RowView<T, VEC>::VN;
-    constexpr int U = VEC ? 4 : 8;        // loads in flight for each thread
+    constexpr int U = VEC && !WIDE ? 4 : 8;     // loads in flight for each thread
     __shared__ Shared<T, NW> shared[kRowsPerBlock];
     const int lane = threadIdx.x & 31;
     const int warp = NW == 1 ? 0 : threadIdx.x >> 5;
@@ -799,6 +800,7 @@ constexpr int64_t kMaxGrid = 1 << 30;
 // 12), else what gives each thread of such a block less than 16 bytes (64 x
 // 2000 f32 with 8 alternatives: 8.2 us, in blocks 6.2).
 constexpr int kWarpRowBytes = 16384, kWarpRow = 1024;
+constexpr int kWideRow = 16384;     // shortest row with eight loads in flight
 // Longest row of the gradient that one warp takes: 4096 x 2000 f32 13 us, in
 // blocks 27; 4096 x 4096 29 us, in blocks 27.
 constexpr int kGradWarpRow = 2048;
@@ -917,7 +919,7 @@ int row_output(const kx_tensor *t, const kx_tensor *logits, uint32_t es, const c
 
 template <typename T, bool VEC, bool ENT>
 void launch_forward(Handle *h, ForwardParams<T> &p) {
-    const int64_t at_once = (int64_t)kBlocks<T, 8> * h->sm_count;
+    const int64_t at_once = (int64_t)kBlocks<T, 8, false> * h->sm_count;
     const bool many = p.rows.count > at_once;
     if (p.len <= (many ? kWarpRowBytes / (int)sizeof(T) : kWarpRow)) {
         const int64_t blocks = (p.rows.count + 3) / 4;
@@ -931,10 +933,26 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     // More rows than that go to blocks of four warps: twice as many rows are on
     // their way at once while others end (4096 x 16384 with 20 alternatives:
     // 60 us, with eight warps 67; 600 x 65536: 36 us, with eight warps 30).
+    // Long f32 rows have eight loads of each thread in flight, with eight such
+    // blocks on an SM instead of ten, unless more places would stay empty in the
+    // last round of rows than that gains (about 7 %): 1000 x 131072 with 8
+    // alternatives 88 us, with four loads 94; 1300 x 50021 59 and 51; 4096 x
+    // 10000 45 and 41.
     if (many) {
-        log_probs_kernel<T, VEC, ENT, 4>
-            <<<(unsigned)std::min<int64_t>(p.rows.count, kMaxGrid), 128, 0, h->stream>>>(p);
         h->last_kernel = "log_probs_block4";
+        const unsigned grid = (unsigned)std::min<int64_t>(p.rows.count, kMaxGrid);
+        if constexpr (sizeof(T) == 4 && VEC) {
+            auto places = [&](int blocks) {
+                const int64_t n = (int64_t)blocks * h->sm_count;
+                return (p.rows.count + n - 1) / n * n;
+            };
+            if (p.len >= kWideRow && places(kBlocks<T, 4, true>) * 100 <= places(kBlocks<T, 4, false>) * 107) {
+                log_probs_kernel<T, VEC, ENT, 4, true><<<grid, 128, 0, h->stream>>>(p);
+                h->last_kernel = "log_probs_block4_wide";
+                return;
+            }
+        }
+        log_probs_kernel<T, VEC, ENT, 4><<<grid, 128, 0, h->stream>>>(p);
         return;
     }
     while (p.cluster < kMaxCluster) {

@@ -100,6 +100,7 @@ def test_layouts(kx, torch_cuda, dtype):
     outs += [buf[20_000 + 1000 * i + 2 * i + 1:][:a.size] for i, a in enumerate(arrs[5:11])]
     outs.append(kx.TensorView(buf, (20, 30), (-1, 20), 40_019))
     norm = kx.clip_grad_norm_into(views, 2.5, outs)
+    assert torch.equal(norm, kx.grad_norm(views))      # the same bits, whatever the outputs are
     host = buf.cpu().numpy()
     last = np.array([[host[40_019 - i + 20 * j] for j in range(30)] for i in range(20)])
     check_clip(norm, outs[:-1] + [torch.from_numpy(last)], arrs, 2.5, dtype)

@@ -183,18 +183,22 @@ def test_masks_ties_and_special_values(kx, torch_cuda, dtype, v):
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 @pytest.mark.parametrize("rows,v,kernel", [
     (5, 301, "log_probs_warp"), (2100, 77, "log_probs_warp"), (760, 1501, "log_probs_warp"),
-    (2050, 2048, "log_probs_warp"), (760, 5001, "log_probs_block4"), (150, 9001, "log_probs_block8"),
+    (2050, 2048, "log_probs_warp"), (760, 5001, "log_probs_block4"),
+    (760, 16_401, "log_probs_block4_wide"), (150, 9001, "log_probs_block8"),
     (40, 1025, "log_probs_block8"), (200, 40001, "log_probs_cluster"), (3, 300_007, "log_probs_cluster"), (1, 1_300_001, "log_probs_cluster")])
 def test_each_kernel_and_strides(kx, torch_cuda, dtype, rows, v, kernel):
     """Rows of every kernel, as rows and with the vocabulary's stride above one;
     the longest make a part of a thread's elements several rounds."""
     torch = torch_cuda
+    if dtype == np.float64 and kernel == "log_probs_block4_wide":
+        kernel = "log_probs_block4"
     x, tokens = logits(13 + v, rows, v, dtype)
     some = np.unique(np.linspace(0, rows - 1, 12).astype(int))
     dx, dt = torch.from_numpy(x).cuda(), torch.from_numpy(tokens).cuda()
     for view in (dx, dx.t().contiguous().t()):
         res = kx.token_log_probs(view, dt, top=32, entropy=True)
-        assert kx.handle(0).last_kernel == kernel
+        assert kx.handle(0).last_kernel == (kernel if view is dx or kernel != "log_probs_block4_wide" else
+                                            "log_probs_block4")
         res = numpy(kx, res, rows)
         check_forward(kx.TokenLogProbs(*[a[some] for a in res]), x[some], tokens[some], 1.0, dtype, 32)
         if view is dx:
@@ -204,7 +208,7 @@ def test_each_kernel_and_strides(kx, torch_cuda, dtype, rows, v, kernel):
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
-@pytest.mark.parametrize("rows,v", [(3, 70_001), (770, 4500), (2080, 2000), (64, 1500)])
+@pytest.mark.parametrize("rows,v", [(3, 70_001), (770, 4500), (770, 17_003), (2080, 2000), (64, 1500)])
 def test_ties_and_masks_in_each_kernel(kx, torch_cuda, dtype, rows, v):
     """Rows of equal values, of few values, with one or no token left, most of
     them masked, in turn."""
