@@ -340,7 +340,7 @@ constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 && 
 // maximum of its elements and the two sums against it; they meet by shuffles,
 // then in shared memory, then (few rows) in that of the cluster's first block,
 // so that one launch and no workspace do for any number of rows.  The bound is
-// the reading of the logits: 4096 x 32000 f32 with entropies takes 85 us, 6.1
+// the reading of the logits: 4096 x 32000 f32 with entropies takes 83 us, 6.3
 // TB/s; in f64 it is the 64-bit pipe, 46 % busy over the 53 us of 509 x 32003,
 // where more registers would be needed to keep it fed.  Few rows wait for one
 // memory round trip after another: 1 x 32000 f32 takes 5.8 us, with
@@ -349,9 +349,9 @@ constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 && 
 // The alternatives come from the threads' maxima: the K-th largest of them, or
 // less, bounds the K-th alternative from below, so only elements at or above
 // it matter.  Threads whose maximum reaches it (a few times K) read the parts
-// of theirs again whose own maxima do, about 5 % of the row: going over all of
-// their elements took 97 us where this takes 72 (1501 x 50021 f32, 8
-// alternatives, half of the tokens masked).  A few dozen candidates are ranked
+// of theirs again whose own maxima do, about 4 % of the row: going over all of
+// their elements took 97 us where this took 72, and takes 63 now (1501 x 50021
+// f32, 8 alternatives, half of the tokens masked).  A few dozen candidates are ranked
 // by counting.  Should more than kCandidates elements reach the bound (rows of
 // equal values), the alternatives are found one after another instead.
 template <typename T, bool VEC, bool ENT, int NW, bool WIDE = false>
