@@ -610,6 +610,40 @@ class _Operands:
         return self.at + off
 
 
+@functools.lru_cache(maxsize=1)
+def _native():
+    """The binding for plain torch tensors (csrc/kx_torch.cpp); it gives None
+    for what it does not take."""
+    import torch  # noqa: F401  (the binding's symbols)
+    from . import _kx_torch
+    names = [f"kx_{n}_{k}" for n in ("token_log_probs", "token_log_probs_backward", "grad_norm", "clip_grad_norm")
+             for k in ("f32", "f64")]
+    _kx_torch.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in (*names, "kx_grad_norm_workspace")])
+    return _kx_torch
+
+
+def _try_native(call, t, *args):
+    """``call`` of the binding in a turn of t's handle, and its results; None
+    where the general path is to take the call or to refuse it."""
+    dev = getattr(t, "get_device", _nowhere)()
+    if dev < 0:
+        return None
+    h = _route(t)
+    err = KxError()
+    with h._turn:
+        h.set_stream(_current_stream(dev))
+        got = call(h._h.value, dev, *args, C.addressof(err))
+    if got is None:
+        return None
+    if got[0]:
+        raise_for(got[0], err)
+    return got[1:]
+
+
+def _nowhere() -> int:
+    return -1
+
+
 def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int = 0,
                     entropy: bool = False) -> TokenLogProbs:
     """Log probabilities of given tokens under ``softmax(logits / temperature)``
@@ -629,6 +663,10 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
     op, dtype, top = "token_log_probs", logits.dtype, int(top)
     if not 0 <= top <= MAX_ALTERNATIVES:
         raise InvalidParameter(f"{op}: top (0 to {MAX_ALTERNATIVES} alternatives)", operation=op, parameter="top")
+    temperature = float(temperature)
+    got = _try_native(_native().token_log_probs, logits, logits, tokens, temperature, top, entropy)
+    if got is not None:
+        return TokenLogProbs._make(got)
     fn = _fn("kx_token_log_probs", dtype)
     h = _route(logits)
     o = _Operands(op, h.device, 7)
@@ -652,7 +690,7 @@ def token_log_probs(logits, tokens=None, *, temperature: float = 1.0, top: int =
         dims, strides = values.shape, values.stride()
         top_lp = o.fresh(values.data_ptr(), count * top, dims, strides)
         top_ids = o.fresh(ids.data_ptr(), count * top, dims, strides)
-    _enqueue(h, fn, *given, float(temperature), lp, lse, ent, top_lp, top_ids)
+    _enqueue(h, fn, *given, temperature, lp, lse, ent, top_lp, top_ids)
     kept = kept.unbind(0)
     return TokenLogProbs(kept[-1] if tokens is not None else None, kept[0], kept[1] if entropy else None, values, ids)
 
@@ -680,6 +718,10 @@ def token_log_probs_backward(logits, tokens=None, *, lse, entropy=None, grad_log
     ``lse`` and (with ``grad_entropy``) ``entropy`` are the forward call's, for
     the same logits and temperature; incoming gradients have their outputs'
     dims (any strides), and one that is None counts as zero."""
+    got = _try_native(_native().token_log_probs_backward, logits, logits, tokens, lse, entropy, grad_log_probs,
+                      grad_entropy, grad_lse, float(temperature), None)
+    if got is not None:
+        return got[0]
     out = getattr(logits, "buffer", logits).new_empty(tuple(logits.shape))
     token_log_probs_backward_into(logits, tokens, out, lse=lse, entropy=entropy, grad_log_probs=grad_log_probs,
                                   grad_entropy=grad_entropy, grad_lse=grad_lse, temperature=temperature)
@@ -690,6 +732,9 @@ def token_log_probs_backward_into(logits, tokens, out, *, lse, entropy=None, gra
                                   grad_lse=None, temperature: float = 1.0) -> None:
     """``token_log_probs_backward`` written into an existing C-contiguous tensor."""
     import torch
+    if _try_native(_native().token_log_probs_backward, logits, logits, tokens, lse, entropy, grad_log_probs,
+                   grad_entropy, grad_lse, float(temperature), out) is not None:
+        return
     dtype = logits.dtype
     fn = _fn("kx_token_log_probs_backward", dtype)
     h = _route(logits)
@@ -768,6 +813,11 @@ def _norm_workspace() -> int:
 
 def _norm_call(op: str, grads, outs, max_norm, norm):
     import torch
+    if grads:
+        max_norm = 0.0 if outs is None else float(max_norm)
+        got = _try_native(_native().grad_norm, grads[0], grads, outs, max_norm, norm)
+        if got is not None:
+            return got[0]
     dtype, arrays = _lists(op, grads, outs)
     fn = _fn("kx_" + op, dtype)
     h = _route(grads[0])
@@ -782,7 +832,7 @@ def _norm_call(op: str, grads, outs, max_norm, norm):
     if outs is None:
         _enqueue(h, fn, arrays[0], n, *tail)
     else:
-        _enqueue(h, fn, arrays[0], n, float(max_norm), arrays[1], *tail)
+        _enqueue(h, fn, arrays[0], n, max_norm, arrays[1], *tail)
     return norm
 
 

@@ -1,13 +1,17 @@
 """Build the sm_100a shared library in-tree with nvcc.
 
 The library is self-contained (static CUDA runtime) and is written next to this
-file as ``libkernix_b200.so`` so that it travels with the source tree.
+file as ``libkernix_b200.so`` so that it travels with the source tree.  The
+binding of the Python mirror's calls on torch tensors, which knows torch and
+nothing of CUDA, is written beside it as ``_kx_torch.so``.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -16,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = ROOT / "_build" / "kernix_b200"
 LIB = PKG / "libkernix_b200.so"
+BINDING = PKG / "_kx_torch.so"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -64,7 +69,25 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB)
+    _binding(force, verbose)
     return LIB
+
+
+def _binding(force: bool, verbose: bool) -> None:
+    """Compile csrc/kx_torch.cpp against the installed torch."""
+    src = CSRC / "kx_torch.cpp"
+    if not force and not _stale(BINDING, [src] + _headers()):
+        return
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden",
+           "-I", sysconfig.get_paths()["include"], "-isystem", str(torch / "include"), "-isystem",
+           str(torch / "include" / "torch" / "csrc" / "api" / "include"), str(src), "-o", str(tmp),
+           "-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
 
 
 if __name__ == "__main__":

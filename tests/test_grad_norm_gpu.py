@@ -7,6 +7,8 @@ bits, so the sum is off by at most n 2^-53 of itself and the root by half of
 that; the norm then rounds once (u).  A scaled element is g times a factor that
 is off by n 2^-53 + 2u, rounded once more: 3u + n 2^-53 of its size, or half a
 step of the smallest numbers."""
+import gc
+
 import numpy as np
 import pytest
 
@@ -339,3 +341,62 @@ def test_calls_of_several_threads(kx, torch_cuda):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_the_binding_and_the_general_path_agree(kx, torch_cuda, monkeypatch):
+    """Every call on torch tensors through csrc/kx_torch.cpp and without it: the
+    same bits, the same refusals, and nothing kept after the call."""
+    torch = torch_cuda
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(4, 7, 333, generator=gen, device="cuda").transpose(0, 1)
+    t = torch.randint(-1, 333, (7, 4), generator=gen, device="cuda")
+    g = torch.randn(4, 7, generator=gen, device="cuda").t()
+    grads = [torch.randn(33, 20, generator=gen, device="cuda").t(), torch.randn(0, 4, device="cuda"),
+             torch.randn(10_001, generator=gen, device="cuda")[1:], torch.randn(6, 8, device="cuda")[:, ::3]]
+
+    def calls():
+        out = kx.token_log_probs(x, t, temperature=0.7, top=5, entropy=True)
+        bare = kx.token_log_probs(x)
+        back = kx.token_log_probs_backward(x, t, lse=out.lse, entropy=out.entropy, grad_log_probs=g, grad_entropy=g,
+                                           grad_lse=g, temperature=0.7)
+        into = torch.empty_like(back)
+        kx.token_log_probs_backward_into(x, t, into, lse=out.lse, grad_log_probs=g, temperature=0.7)
+        norm, clipped = kx.clip_grad_norm(grads, 0.5)
+        mine = [q.clone() for q in grads]
+        again = torch.zeros(1, device="cuda")
+        kx.clip_grad_norm_into(mine, 0.5, mine, again)
+        assert bare.log_probs is None and bare.entropy is None and bare.top_tokens is None
+        return [*out, bare.lse, back, into, norm, kx.grad_norm(grads), *clipped, *mine, again]
+
+    def refusals():
+        got = []
+        for call in (lambda: kx.token_log_probs(x, t[:3]), lambda: kx.token_log_probs(x, t, temperature=-1.0),
+                     lambda: kx.token_log_probs(x, t.int()), lambda: kx.token_log_probs(x.half(), t),
+                     lambda: kx.token_log_probs_backward(x, t, lse=g.double(), grad_log_probs=g),
+                     lambda: kx.token_log_probs_backward_into(x, t, x, lse=g, grad_log_probs=g),
+                     lambda: kx.grad_norm([x, g.double()]), lambda: kx.grad_norm([x, t]),
+                     lambda: kx.clip_grad_norm_into([x, g], 1.0, [x]), lambda: kx.clip_grad_norm_into([x], 1.0, [g]),
+                     lambda: kx.clip_grad_norm([x], float("nan")), lambda: kx.clip_grad_norm_into([g, g], 1.0, [g, g]),
+                     lambda: kx.grad_norm_into([x], torch.zeros(2, device="cuda"))):
+            with pytest.raises(kx.OpsError) as e:
+                call()
+            got.append((type(e.value), e.value.fields))
+        return got
+
+    native, refused = calls(), refusals()
+    gc.collect()        # what the refusals' tracebacks hold
+    held = torch.cuda.memory_allocated()
+    for _ in range(50):
+        calls()
+        refusals()
+    gc.collect()
+    assert torch.cuda.memory_allocated() == held
+
+    class Nothing:
+        token_log_probs = token_log_probs_backward = grad_norm = staticmethod(lambda *a: None)
+
+    monkeypatch.setattr(kx, "_native", lambda: Nothing)
+    general = calls()
+    assert all(torch.equal(a, b) and a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride()
+               for a, b in zip(native, general))
+    assert refusals() == refused

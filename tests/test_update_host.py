@@ -225,3 +225,28 @@ def test_lists_describe_contiguous_pairs_by_their_elements():
     assert (arr[2].rank, arr[2].dims[0]) == (1, 0) and (arr[3].rank, arr[3].dims[0]) == (1, 1)
     arr = kx._descriptors(o, alone)
     assert list(arr[4].strides)[:2] == [1, 2]
+
+
+def test_the_binding_leaves_what_it_does_not_take():
+    """kernix_b200._kx_torch on the host: anything but CUDA tensors of one
+    device and dtype is left to the general path, with nothing called."""
+    import torch
+
+    native = kx._native()
+    x, t = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64)
+    err = _abi.KxError()
+    h, e = C.addressof(FAKE), C.addressof(err)
+    assert native.token_log_probs(h, 0, x, t, 1.0, 0, False, e) is None
+    assert native.token_log_probs(h, 0, "x", t, 1.0, 0, False, e) is None
+    view = kx.TensorView(torch.zeros(10), (2, 5), (5, 1))
+    assert native.token_log_probs_backward(h, 0, view, None, x, None, x, None, None, 1.0, None, e) is None
+    assert native.grad_norm(h, 0, [], None, 0.0, None, e) is None
+    assert native.grad_norm(h, 0, [x], None, 0.0, None, e) is None
+    assert native.grad_norm(h, 0, (x,), None, 0.0, None, e) is None
+    for name, count in (("token_log_probs", 8), ("token_log_probs_backward", 12), ("grad_norm", 7), ("bind", 9)):
+        with pytest.raises(TypeError):
+            getattr(native, name)(*[0] * (count - 1))
+    with pytest.raises(ValueError):
+        native.bind(*[0] * 9)
+    with pytest.raises(TypeError):
+        native.token_log_probs("h", 0, x, t, 1.0, 0, False, e)
