@@ -386,11 +386,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
         const RowView<T, VEC> x(p.x + row_offset(p.rows, kLogits, row), p.len, p.stride);
         // the given token's logit, on its way while the row is read
         int64_t token = -1;
-        T given = T(NAN);
-        if (p.log_probs && rank == 0 && tid == 0) {
-            token = p.tokens[row_offset(p.rows, kTokens, row)];
-            if (token >= 0 && token < p.len) given = x.at((int)token);
-        }
+        if (p.log_probs && rank == 0 && tid == 0) token = p.tokens[row_offset(p.rows, kTokens, row)];
         const int per = (x.nv + C - 1) / C;
         const int v0 = min(rank * per, x.nv), v1 = min(v0 + per, x.nv);
         const bool edges = VEC && rank == 0 && warp == 0;   // the warp of the head and the tail
@@ -420,6 +416,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
             const T v[1] = {lane >= 16 && lane < 16 + x.tail ? x.at(tail0 + lane - 16) : T(-INFINITY)};
             st.add(v, c, ex);
         }
+        // its logit, now that asking for it holds up no load of the row
+        const T given = token >= 0 && token < p.len ? x.at((int)token) : T(NAN);
         const T mine = st.m;
         st.template join<32>(c, ex);
         T bound = lowest<T>();
@@ -496,12 +494,20 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
             const int n = sh.found;
             if (n <= kCandidates<NW>) {
                 for (int k = n + tid; k < p.top; k += GT) sh.best[k] = Key<T>::none(32 * rank + k);
-                for (int k = tid; k < n; k += GT) {
-                    const Key<T> mine_k = sh.cand[k];
+                // Four lanes for each candidate where a row has eight warps (509
+                // x 32003 f64, 4 alternatives: 44.8 us, one lane 46.8; four warps
+                // have rows enough to wait for, and 85.7 us for the 79.6 of 4096
+                // x 32000 f32 with the code of it in their kernel).
+                constexpr int kLanes = NW == 8 ? 4 : 1;
+                for (int k0 = tid / 32 * (32 / kLanes); k0 < n; k0 += GT / kLanes) {
+                    const int k = k0 + lane / kLanes;
+                    const Key<T> mine_k = sh.cand[min(k, n - 1)];
                     int place = 0;
 #pragma unroll 8
-                    for (int o = 0; o < n; ++o) place += sh.cand[o].before(mine_k);
-                    if (place < p.top) sh.best[place] = mine_k;
+                    for (int o = lane % kLanes; o < n; o += kLanes) place += sh.cand[o].before(mine_k);
+#pragma unroll
+                    for (int o = 1; o < kLanes; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+                    if (lane % kLanes == 0 && k < n && place < p.top) sh.best[place] = mine_k;
                 }
             } else {
                 Key<T> last = Key<T>::first();
@@ -582,7 +588,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
                     // each come before this one, by halving, in all at once
                     key = sh.list[k / p.top][k % p.top];
                     int less[kMaxCluster] = {};
-                    for (int by = 32; by > 0; by >>= 1) {
+#pragma unroll 1
+                    for (int by = 1 << (31 - __clz(p.top)); by > 0; by >>= 1) {
 #pragma unroll
                         for (int l = 0; l < kMaxCluster; ++l) {
                             const int to = less[l] + by;
