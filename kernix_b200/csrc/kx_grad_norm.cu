@@ -292,10 +292,13 @@ constexpr uint64_t kMostTensors = 1u << 20;
 constexpr int64_t kCount32 = 1ll << 31;    // 32 bits count fewer elements, and a block's step beyond them
 constexpr int64_t kFold = 2048;        // most partial sums that each block of the scaling adds
 
-// Bytes of gradients up to which the scaling marks its accesses as the first to
-// leave the cache (of 126 MB): of 64 MB clipping takes 32.5 us, without 35.2; of
-// 256 MB 132 and 133.5; of 1 GB 525 and 514.
-constexpr int64_t kShortly = 256ll << 20;
+// Bytes of gradients between which the scaling marks its accesses as the first to
+// leave the cache of 126 MB: 48 MB are clipped in 25.9 us, without marks in 28.5,
+// 64 MB in 32.5 and 35.3, 128 MB in 62.0 and 65.6.  Fewer have room beside their
+// copies, which are there for who reads them next (clipped and read, 44 MB take
+// 34.7 and 33.2, 48 MB 37.1 and 37.6); of more little is left to read again (192
+// MB clipped and read: 134.9 both ways, 256 MB 179 and 176).
+constexpr int64_t kShortlyFrom = 46ll << 20, kShortlyTo = 192ll << 20;
 
 constexpr uint64_t kWorkspace = (1 + kRoom) * sizeof(double);
 
@@ -544,8 +547,9 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
         to = nullptr;
     }
     if (outs) {
+        const bool shortly = bytes > kShortlyFrom && bytes <= kShortlyTo;
         for (const Batch<T> &b : batches) {
-            launch_after(h, bytes <= kShortly ? scale_spans_kernel<T, true> : scale_spans_kernel<T, false>, b.blocks(h),
+            launch_after(h, shortly ? scale_spans_kernel<T, true> : scale_spans_kernel<T, false>, b.blocks(h),
                          b.spans, b.outs, sums, used, max_norm, to);
             to = nullptr;
         }

@@ -3,7 +3,7 @@
 //
 // Those calls have many small operands, or long lists of them, beside a kernel
 // of a few microseconds: from Python a call with 6 operands took 25 us and a
-// list of 56 gradients and outputs 69, most of it in reading attributes one by
+// list of 38 gradients and outputs 69, most of it in reading attributes one by
 // one.  Everything that is refused or out of the ordinary (descriptors that are
 // not tensors, other devices or dtypes) gives None here, and the caller's own
 // path says why or takes it.

@@ -159,6 +159,36 @@ def test_more_elements_than_32_bits_count(kx, torch_cuda):
     assert float(x.min()) == float(x.max())
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("megabytes", [45, 47, 100, 191, 193])
+def test_lists_of_the_size_of_the_cache(kx, torch_cuda, dtype, megabytes):
+    """Lists that the second-level cache holds partly, with unaligned and tiny
+    members: copies apart and in place have the same bits, and every element is
+    its gradient's, scaled."""
+    torch = torch_cuda
+    ty = torch.float32 if dtype == np.float32 else torch.float64
+    size = 4 if dtype == np.float32 else 8
+    gen = torch.Generator(device="cuda").manual_seed(megabytes)
+    each = megabytes * 2 ** 20 // size // 4
+    base = [torch.randn(each + 3, generator=gen, device="cuda", dtype=ty) for _ in range(4)]
+    grads = [base[0][:each], base[1][1:each], base[2][3:], base[3][:each - 2], base[0][each:], base[3][each:each + 1]]
+    outs = [torch.full((g.numel() + 9,), 7.0, device="cuda", dtype=ty) for g in grads]
+    views = [o[4:4 + g.numel()] if i != 2 else o[:g.numel()] for i, (o, g) in enumerate(zip(outs, grads))]
+    norm = kx.clip_grad_norm_into(grads, 2.5, views)
+    n = sum(g.numel() for g in grads)
+    want = float(torch.stack([g.double().square().sum() for g in grads]).sum().sqrt())
+    # n squares added up here and there, in any order: each sum is off by n 2^-53 of itself
+    assert abs(float(norm) - want) <= want * (U[dtype] + 2 * n * 2.0 ** -53)
+    by = 2.5 / want
+    for i, (g, v, o) in enumerate(zip(grads, views, outs)):
+        error = (v.double() - g.double() * by).abs()
+        assert bool((error <= g.double().abs() * by * (3 * U[dtype] + 2 * n * 2.0 ** -53)).all())
+        rest = [o[:4], o[4 + g.numel():]] if i != 2 else [o[g.numel():]]
+        assert all(bool((r == 7.0).all()) for r in rest)
+    assert torch.equal(kx.clip_grad_norm_into(grads, 2.5, grads), norm)
+    assert all(torch.equal(g, v) for g, v in zip(grads, views))
+
+
 @pytest.mark.parametrize("count,rows", [(6, 1100), (45, 1100), (300, 3)])
 def test_many_tensors_with_gaps(kx, torch_cuda, count, rows):
     """Lists whose partial sums are folded before the scaling, and on the way."""
