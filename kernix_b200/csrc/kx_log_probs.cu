@@ -340,11 +340,13 @@ constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 && 
 // maximum of its elements and the two sums against it; they meet by shuffles,
 // then in shared memory, then (few rows) in that of the cluster's first block,
 // so that one launch and no workspace do for any number of rows.  The bound is
-// the reading of the logits: 4096 x 32000 f32 with entropies takes 83 us, 6.3
-// TB/s; in f64 it is the 64-bit pipe, 46 % busy over the 53 us of 509 x 32003,
-// where more registers would be needed to keep it fed.  Few rows wait for one
-// memory round trip after another: 1 x 32000 f32 takes 5.8 us, with
-// alternatives 8 to 9.
+// the reading of the logits: 4096 x 32000 f32 with entropies takes 80 us, 6.5
+// TB/s; in f64 it is arithmetic, 48 instructions for an element of which the
+// 64-bit pipe takes 17: 509 x 32003 takes 45 us.  (Copies into shared memory two
+// steps ahead, with half as many elements of a thread at a time, took 61: what
+// keeps the pipe busy is the number of independent exponentials.)  Few rows wait
+// for one memory round trip after another: 1 x 32000 f32 takes 3.7 us, with
+// alternatives 5.8 to 6.4.
 //
 // The alternatives come from the threads' maxima: the K-th largest of them, or
 // less, bounds the K-th alternative from below, so only elements at or above
@@ -924,6 +926,11 @@ int row_output(const kx_tensor *t, const kx_tensor *logits, uint32_t es, const c
     return seen->add(t, s, es, true, op, err);
 }
 
+// Elements from which on another part of a row is worth its merging where the
+// device has room for both: 296 x 17000 f64 with 8 alternatives takes 22.5 us in
+// two parts, 19.3 in one.
+template <typename T> constexpr int kLongPart = sizeof(T) == 4 ? 16384 : 12288;
+
 template <typename T, bool VEC, bool ENT>
 void launch_forward(Handle *h, ForwardParams<T> &p) {
     const int64_t at_once = (int64_t)kBlocks<T, 8, false> * h->sm_count;
@@ -936,7 +943,8 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     }
     // Rows that blocks of eight warps take at once have one each, or a cluster:
     // for the SMs that would have nothing (1 x 131072 f32: 6 us in eight parts,
-    // 16 in one), or for long parts (64 x 131072: 10 us, with four parts 12).
+    // 16 in one), or for long parts (64 x 131072: 10 us, with four parts 12; 200 x
+    // 32003 f64 with 8 alternatives: 24.7 us, in one part 27.4).
     // More rows than that go to blocks of four warps: twice as many rows are on
     // their way at once while others end (4096 x 16384 with 20 alternatives:
     // 60 us, with eight warps 67; 600 x 65536: 36 us, with eight warps 30).
@@ -964,7 +972,7 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     }
     while (p.cluster < kMaxCluster) {
         const int64_t blocks = p.rows.count * p.cluster, piece = p.len / (2 * p.cluster);
-        if (!(blocks < h->sm_count && piece >= 4096) && !(2 * blocks <= at_once && piece >= 16384)) break;
+        if (!(blocks < h->sm_count && piece >= 4096) && !(2 * blocks <= at_once && piece >= kLongPart<T>)) break;
         p.cluster *= 2;
     }
     cudaLaunchConfig_t cfg = {};
