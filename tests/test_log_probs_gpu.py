@@ -207,6 +207,19 @@ def test_each_kernel_and_strides(kx, torch_cuda, dtype, rows, v, kernel):
     assert np.array_equal(first.top_tokens, res.top_tokens)
 
 
+@pytest.mark.parametrize("dtype,v,kernel", [
+    (np.float64, 24_575, "log_probs_block8"), (np.float64, 24_577, "log_probs_cluster"),
+    (np.float32, 32_767, "log_probs_block8"), (np.float32, 32_769, "log_probs_cluster")])
+def test_rows_in_two_parts(kx, torch_cuda, dtype, v, kernel):
+    """From which length on rows that the SMs have places for twice are cut."""
+    rows = torch_cuda.cuda.get_device_properties(0).multi_processor_count + 2
+    x, tokens = logits(v, rows, v, dtype)
+    res = run(kx, torch_cuda, x, tokens, 0.9, 6)
+    assert kx.handle(0).last_kernel == kernel
+    some = np.array([0, 1, 73, rows - 1])
+    check_forward(kx.TokenLogProbs(*[a[some] for a in res]), x[some], tokens[some], 0.9, dtype, 6)
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 @pytest.mark.parametrize("rows,v", [(3, 70_001), (770, 4500), (770, 17_003), (2080, 2000), (64, 1500)])
 def test_ties_and_masks_in_each_kernel(kx, torch_cuda, dtype, rows, v):
