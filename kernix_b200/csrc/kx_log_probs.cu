@@ -991,6 +991,26 @@ void launch_forward(Handle *h, ForwardParams<T> &p) {
     h->last_kernel = p.cluster > 1 ? "log_probs_cluster" : "log_probs_block8";
 }
 
+// Into how many parts the gradient cuts a row: `wanted` or a few more, so that
+// the last round of blocks is short or full, where each part costs the time of
+// 13 KB beside its own elements (300 x 40000 f64: 42 us, in two parts 51; 700 x
+// 20011 f64 52 and 57, f32 23 and 24; with 8 KB 2000 x 9000 f64 would be cut in two:
+// 68 us, whole 63).
+template <typename T> int parts_of_least_time(const Handle *h, int64_t rows, int64_t len, int64_t wanted) {
+    const int64_t places = (int64_t)kGradBlocks * h->sm_count, most = std::max<int64_t>(1, len / kGradPartLeast);
+    const int64_t from = std::min(std::max<int64_t>(1, wanted), most), to = std::min(from + 3, most);
+    int64_t parts = from, least = INT64_MAX;
+    for (int64_t n = from; n <= to; ++n) {
+        const int64_t rounds = (rows * n + places - 1) / places;
+        const int64_t time = rounds * (len / n + 13 * 1024 / (int64_t)sizeof(T));
+        if (time < least) {
+            least = time;
+            parts = n;
+        }
+    }
+    return (int)parts;
+}
+
 template <typename T, bool VEC, int NW> void launch_backward(Handle *h, const BackwardParams<T> &p) {
     constexpr int kGroups = kGradThreads / (NW * 32);
     const i128 groups = (i128)p.rows.count * p.parts;
@@ -1155,9 +1175,9 @@ int backward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *token
         vec ? launch_backward<T, true, 1>(h, p) : launch_backward<T, false, 1>(h, p);
     } else {
         // even parts, as many as the device takes at once, or of the longest size
-        const int64_t wanted = std::max<int64_t>(kGradBlocks * h->sm_count / p.rows.count,
+        const int64_t wanted = std::max<int64_t>((int64_t)kGradBlocks * h->sm_count / p.rows.count,
                                                  (p.len + kGradPartMost - 1) / kGradPartMost);
-        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(wanted, p.len / kGradPartLeast));
+        p.parts = parts_of_least_time<T>(h, p.rows.count, p.len, wanted);
         p.per = ((p.len + p.parts - 1) / p.parts + 15) / 16 * 16;
         p.parts = (p.len + p.per - 1) / p.per;
         vec ? launch_backward<T, true, kGradThreads / 32>(h, p) : launch_backward<T, false, kGradThreads / 32>(h, p);
