@@ -757,10 +757,10 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
 
 // The gradient: one element in, one out, with a row's few numbers between
 // them.  The bound is the two streams: 4096 x 32000 f32 takes 165 us, 6.4
-// TB/s, and 169 where the two lie differently against 16 bytes.  A block takes a part of one row: parts of 32000 elements there, where
-// parts of 8192 took 190 us and of 2048 343, as each begins with its row's
-// numbers; or each of its warps a short row (4096 x 1000: 8 us, with a block
-// for each row 23).
+// TB/s, and 169 where the two lie differently against 16 bytes.  A block takes a
+// part of one row: parts of 32000 elements there, where parts of 8192 took 190 us
+// and of 2048 343, as each begins with its row's numbers; or each of its warps a
+// short row (4096 x 1000: 8 us, with a block for each row 23).
 template <typename T, bool VEC, int NW>
 __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
     log_probs_backward_kernel(const __grid_constant__ BackwardParams<T> p) {
@@ -817,8 +817,8 @@ constexpr int kWideRow = 16384;     // shortest row with eight loads in flight
 constexpr int kGradWarpRow = 2048;
 // Elements of a block's part of a row in the gradient: no fewer, for the few
 // rows that are cut for the SMs' sake (8 x 30208 f32: 5.5 us, in parts of 16384
-// 7.5), and no more, for the last blocks to end together (1501 x 50021: 103 us,
-// whole rows 108).
+// 7.5), and no more, for the last blocks to end together (2000 x 100000: 247 us,
+// whole rows 257).
 constexpr int kGradPartLeast = 4096, kGradPartMost = 32768;
 // The temperature divides logits: it and its reciprocal are normal numbers.
 template <typename T> bool temperature_ok(T t) {
