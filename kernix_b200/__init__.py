@@ -69,7 +69,7 @@ class Handle:
         raise_for(lib.kx_create(device, C.byref(ptr), C.byref(err)), err)
         self._h = ptr
         self._stream = 0            # the raw stream the library handle orders work on
-        self._turn = threading.Lock()
+        self._turn = threading.RLock()      # again: a finaliser may call while a call of its thread has the turn
 
     @classmethod
     def adopt(cls, ptr: C.c_void_p, device: int) -> "Handle":
@@ -78,7 +78,7 @@ class Handle:
         h.device = device
         h._h = ptr
         h._stream = 0
-        h._turn = threading.Lock()
+        h._turn = threading.RLock()
         return h
 
     @property
@@ -161,7 +161,11 @@ def using(h: Handle):
 
 
 def handle(device: int | None = None) -> Handle:
-    """The per-process default handle of ``device`` (torch's current device by default)."""
+    """The per-process default handle of ``device`` (torch's current device by
+    default).  Threads may share it: each call binds the thread's current
+    stream and enqueues in one turn.  Its scratch (split sums, gathered
+    operands) is one buffer, so products that run at the same time on several
+    streams want a handle each (``using``)."""
     import torch
     if device is None:
         device = torch.cuda.current_device()
@@ -250,10 +254,15 @@ def _route(t) -> Handle:
     return (routed and routed.get(dev)) or _handles.get(dev) or handle(dev)
 
 
-def _bind(t) -> Handle:
-    h = _route(t)
-    h.set_stream(_current_stream(h.device))
-    return h
+def _enqueue(h: Handle, fn, *args) -> None:
+    """The library call ``fn`` on the current stream, in one turn of ``h``:
+    threads that share a handle must not change its stream between the two."""
+    err = KxError()
+    with h._turn:
+        h.set_stream(_current_stream(h.device))
+        rc = fn(h._h, *args, C.byref(err))
+    if rc:
+        raise_for(rc, err)
 
 
 def _empty(dims, dtype, device):
@@ -307,10 +316,9 @@ def matmul(a, b):
 def matmul_into(a, b, out) -> None:
     """Write ``matmul(a, b)`` into an existing C-contiguous device tensor."""
     fn = _fn("kx_matmul", a.dtype)
-    h = _bind(a)
-    err = KxError()
+    h = _route(a)
     da, db, do = _descriptor(a), _descriptor(b), _descriptor(out)
-    raise_for(fn(h.ptr, C.byref(da), C.byref(db), C.byref(do), C.byref(err)), err)
+    _enqueue(h, fn, C.byref(da), C.byref(db), C.byref(do))
 
 
 def matmul_into_replicated(a, b, out, out_mc: int) -> None:
@@ -318,27 +326,29 @@ def matmul_into_replicated(a, b, out, out_mc: int) -> None:
     address of ``out``'s first element: the product lands in the copy of
     ``out`` on every GPU bound to the multicast object."""
     fn = _fn("kx_matmul_replicated", a.dtype)
-    h = _bind(a)
-    err = KxError()
+    h = _route(a)
     da, db, do = _descriptor(a), _descriptor(b), _descriptor(out)
     # out_mc addresses out's first element; the library adds the origin itself
     base = int(out_mc) - do.origin * out.element_size()
-    raise_for(fn(h.ptr, C.byref(da), C.byref(db), C.byref(do), C.c_void_p(base), C.byref(err)), err)
+    _enqueue(h, fn, C.byref(da), C.byref(db), C.byref(do), C.c_void_p(base))
 
 
 class _Ordered:
-    """Run the enclosed device calls of ``h`` in ordered mode."""
+    """Run the enclosed device calls of ``h`` in ordered mode, in one turn of
+    the handle: other threads' calls keep their own mode."""
 
     def __init__(self, h: Handle):
         self.h = h
 
     def __enter__(self):
+        self.h._turn.acquire()
         self.prev = self.h.ordered_matmul
         self.h.set_ordered_matmul(True)
         return self.h
 
     def __exit__(self, *exc):
         self.h.set_ordered_matmul(self.prev)
+        self.h._turn.release()
         return False
 
 
@@ -346,7 +356,7 @@ def matmul_reference(a, b):
     """``matmul_reference`` on the device: every output accumulated in
     increasing k with separately rounded multiply and add (linalg.rs:57-64),
     so the bits equal Kernix's ordered CPU result."""
-    with _Ordered(_bind(a)):
+    with _Ordered(_route(a)):
         return matmul(a, b)
 
 
@@ -394,17 +404,16 @@ def conv2d(x, w, options: Conv2dOptions = Conv2dOptions()):
 def conv2d_into(x, w, out, options: Conv2dOptions = Conv2dOptions()) -> None:
     """``conv2d`` written into an existing C-contiguous device tensor."""
     fn = _fn("kx_conv2d", x.dtype)
-    h = _bind(x)
-    err = KxError()
+    h = _route(x)
     o = options.to_c()
     dx, dw, do = _descriptor(x), _descriptor(w), _descriptor(out)
-    raise_for(fn(h.ptr, C.byref(dx), C.byref(dw), C.byref(o), C.byref(do), C.byref(err)), err)
+    _enqueue(h, fn, C.byref(dx), C.byref(dw), C.byref(o), C.byref(do))
 
 
 def conv2d_reference(x, w, options: Conv2dOptions = Conv2dOptions()):
     """``conv2d_reference`` on the device: the ordered scalar loop
     (neural.rs:188-198, 341-357), bitwise equal to Kernix's CPU result."""
-    with _Ordered(_bind(x)):
+    with _Ordered(_route(x)):
         return conv2d(x, w, options)
 
 
@@ -419,12 +428,11 @@ def tensordot(a, b, a_axes: Sequence[int], b_axes: Sequence[int]):
     ok = len(a_axes) == len(b_axes) and all(-ra <= x < ra for x in a_axes) and all(-rb <= x < rb for x in b_axes)
     out = _empty(tuple(dims) if ok else (), a.dtype, a.device)
     fn = _fn("kx_tensordot", a.dtype)
-    h = _bind(a)
+    h = _route(a)
     la = (C.c_int64 * max(1, len(a_axes)))(*[int(x) for x in a_axes])
     lb = (C.c_int64 * max(1, len(b_axes)))(*[int(x) for x in b_axes])
-    err = KxError()
     ta, tb, to = _descriptor(a), _descriptor(b), _descriptor(out)
-    raise_for(fn(h.ptr, C.byref(ta), C.byref(tb), la, len(a_axes), lb, len(b_axes), C.byref(to), C.byref(err)), err)
+    _enqueue(h, fn, C.byref(ta), C.byref(tb), la, len(a_axes), lb, len(b_axes), C.byref(to))
     return out
 
 
@@ -436,14 +444,13 @@ def matmul_backward(a, b, grad, need_a: bool = True, need_b: bool = True):
     summed back over the batch axes its operand was broadcast along; a
     gradient not asked for is None."""
     fn = _fn("kx_matmul_backward", a.dtype)
-    h = _bind(a)
+    h = _route(a)
     da = _empty(tuple(a.shape), a.dtype, a.device) if need_a else None
     db = _empty(tuple(b.shape), b.dtype, b.device) if need_b else None
-    err = KxError()
     ta, tb, tg = _descriptor(a), _descriptor(b), _descriptor(grad)
     oa = C.byref(_descriptor(da)) if da is not None else None
     ob = C.byref(_descriptor(db)) if db is not None else None
-    raise_for(fn(h.ptr, C.byref(ta), C.byref(tb), C.byref(tg), oa, ob, C.byref(err)), err)
+    _enqueue(h, fn, C.byref(ta), C.byref(tb), C.byref(tg), oa, ob)
     return da, db
 
 
@@ -451,14 +458,12 @@ def conv2d_backward(x, w, grad, options: Conv2dOptions = Conv2dOptions()):
     """conv2d_backward (neural.rs:379-430): (grad_input, grad_weight), bit for
     bit the reference loop's sums."""
     fn = _fn("kx_conv2d_backward", x.dtype)
-    h = _bind(x)
+    h = _route(x)
     dx = _empty(tuple(x.shape), x.dtype, x.device)
     dw = _empty(tuple(w.shape), w.dtype, w.device)
-    err = KxError()
     o = options.to_c()
     tx, tw, tg, ox, ow = (_descriptor(t) for t in (x, w, grad, dx, dw))
-    raise_for(fn(h.ptr, C.byref(tx), C.byref(tw), C.byref(tg), C.byref(o), C.byref(ox), C.byref(ow), C.byref(err)),
-              err)
+    _enqueue(h, fn, C.byref(tx), C.byref(tw), C.byref(tg), C.byref(o), C.byref(ox), C.byref(ow))
     return dx, dw
 
 
@@ -476,10 +481,9 @@ def softmax_temperature(src, axis: int, temperature: float):
 def softmax_temperature_into(src, axis: int, temperature: float, out) -> None:
     """``softmax_temperature`` written into an existing C-contiguous tensor."""
     fn = _fn("kx_softmax_temperature", src.dtype)
-    h = _bind(src)
-    err = KxError()
+    h = _route(src)
     ds, do = _descriptor(src), _descriptor(out)
-    raise_for(fn(h.ptr, C.byref(ds), int(axis), float(temperature), C.byref(do), C.byref(err)), err)
+    _enqueue(h, fn, C.byref(ds), int(axis), float(temperature), C.byref(do))
 
 
 def attention(q, kt, v, temperature: float):
@@ -505,11 +509,9 @@ def attention_into(q, kt, v, temperature: float, out) -> None:
     import torch
     if q.dtype != torch.float32:
         raise Unsupported(f"dtype {q.dtype}: attention runs in f32")
-    h = _bind(q)
-    err = KxError()
+    h = _route(q)
     dq, dk, dv, do = _descriptor(q), _descriptor(kt), _descriptor(v), _descriptor(out)
-    raise_for(lib.kx_attention_f32(h.ptr, C.byref(dq), C.byref(dk), C.byref(dv), float(temperature), C.byref(do),
-                                   C.byref(err)), err)
+    _enqueue(h, lib.kx_attention_f32, C.byref(dq), C.byref(dk), C.byref(dv), float(temperature), C.byref(do))
 
 
 def softmax(src, axis: int):
@@ -523,10 +525,9 @@ def softmax(src, axis: int):
 def softmax_into(src, axis: int, out) -> None:
     """``softmax`` written into an existing C-contiguous tensor."""
     fn = _fn("kx_softmax", src.dtype)
-    h = _bind(src)
-    err = KxError()
+    h = _route(src)
     ds, do = _descriptor(src), _descriptor(out)
-    raise_for(fn(h.ptr, C.byref(ds), int(axis), C.byref(do), C.byref(err)), err)
+    _enqueue(h, fn, C.byref(ds), int(axis), C.byref(do))
 
 
 # ---------------------------------------------------------------------------
@@ -544,17 +545,6 @@ class TokenLogProbs(NamedTuple):
     entropy: "object" = None
     top_log_probs: "object" = None      # [.., top], falling
     top_tokens: "object" = None         # [.., top], int64
-
-
-def _enqueue(h: Handle, fn, *args) -> None:
-    """The library call ``fn`` on the current stream, in one turn: threads that
-    share a handle must not change its stream between the two."""
-    err = KxError()
-    with h._turn:
-        h.set_stream(_current_stream(h.device))
-        rc = fn(h._h, *args, C.byref(err))
-    if rc:
-        raise_for(rc, err)
 
 
 # A kx_tensor of each rank as words: data, storage_len, origin, rank, then dims
@@ -935,7 +925,8 @@ def try_dense_matmul(a: np.ndarray, b: np.ndarray, out: np.ndarray, m: int, k: i
         return False
     h = _host_handle(device)
     fn = getattr(lib, f"kx_try_dense_matmul_{kind}")
-    rc = fn(h.ptr, a.ctypes.data, a.size, b.ctypes.data, b.size, out.ctypes.data, out.size, m, k, n)
+    with h._turn:
+        rc = fn(h.ptr, a.ctypes.data, a.size, b.ctypes.data, b.size, out.ctypes.data, out.size, m, k, n)
     return rc == _abi.KX_OK
 
 
@@ -947,7 +938,8 @@ def try_strided_matmul(a: MatrixInput, b: MatrixInput, out: np.ndarray, device: 
     h = _host_handle(device)
     fn = getattr(lib, f"kx_try_strided_matmul_{kind}")
     ma, mb = a._c(), b._c()
-    rc = fn(h.ptr, C.byref(ma), C.byref(mb), out.ctypes.data, out.size)
+    with h._turn:
+        rc = fn(h.ptr, C.byref(ma), C.byref(mb), out.ctypes.data, out.size)
     return rc == _abi.KX_OK
 
 

@@ -102,14 +102,12 @@ def rows_sharded(a_local, b, out, plan: RowPlan, rank: int, peer_ptrs=None, out_
     last piece) -- enqueued on the current stream."""
     import ctypes as C
 
-    from . import _abi, _bind, _descriptor
-    h = _bind(out)
+    from . import _abi, _descriptor, _enqueue, _route
+    h = _route(out)
     da, db, do = _descriptor(a_local), _descriptor(b), _descriptor(out)
     peers = (C.c_void_p * plan.world)(*peer_ptrs) if peer_ptrs is not None else None
-    err = _abi.KxError()
-    rc = _abi.lib.kx_matmul_rows_sharded_f32(h.ptr, C.byref(da), C.byref(db), C.byref(do), rank, plan.world,
-                                             plan.piece, peers, C.c_void_p(int(out_mc) or None), C.byref(err))
-    _abi.raise_for(rc, err)
+    _enqueue(h, _abi.lib.kx_matmul_rows_sharded_f32, C.byref(da), C.byref(db), C.byref(do), rank, plan.world,
+             plan.piece, peers, C.c_void_p(int(out_mc) or None))
 
 
 def gemm_sharded(handles, a_windows, b_replicas, outs, gather_out: bool = True) -> None:
@@ -119,6 +117,7 @@ def gemm_sharded(handles, a_windows, b_replicas, outs, gather_out: bool = True) 
     ``b_replicas[r]`` B there, ``outs[r]`` a C-contiguous [M, N] output there;
     with ``gather_out`` every output ends with the whole product once each
     handle's stream has completed (``Handle.synchronize``)."""
+    import contextlib
     import ctypes as C
 
     from . import _abi, _descriptor
@@ -130,7 +129,10 @@ def gemm_sharded(handles, a_windows, b_replicas, outs, gather_out: bool = True) 
     db = (_abi.KxTensor * n)(*[_descriptor(t) for t in b_replicas])
     do = (_abi.KxTensor * n)(*[_descriptor(t) for t in outs])
     err = _abi.KxError()
-    rc = _abi.lib.kx_gemm_sharded_f32(hs, n, da, db, do, int(bool(gather_out)), C.byref(err))
+    with contextlib.ExitStack() as turns:
+        for h in sorted(handles, key=id):       # in one order, whoever else takes several
+            turns.enter_context(h._turn)
+        rc = _abi.lib.kx_gemm_sharded_f32(hs, n, da, db, do, int(bool(gather_out)), C.byref(err))
     _abi.raise_for(rc, err)
 
 
