@@ -17,6 +17,7 @@
 #include <climits>
 #include <cmath>
 #include <cstring>
+#include <limits>
 
 #include "kx_internal.hpp"
 
@@ -622,13 +623,21 @@ template <typename T> struct BackwardParams {
     int len, per, parts;     // elements of one block's part of a row; parts of a row
     T factor;                // exp_factor(temperature)
     double temperature, inverse;
+    double trusted;          // lse_trusted(temperature)
+    T before;                // before x after = 1 / temperature
+    double after;
     Rows rows;
 };
 
-// A row's lse is known to half a step of its own size; beyond this size that
-// would show in the probabilities, and the row's maximum and sum are taken
-// anew instead.
-constexpr double kLseTrusted = 256.0;
+// A row's lse is known to half a step of its own size; beyond 256 that would
+// show in the probabilities, and the row's maximum and sum are taken anew
+// instead.  So they are where T lse, which at temperatures near the type's
+// largest number need not be finite in it, is beyond a quarter of that number's
+// last place: a logit of the type's lowest value less T lse is finite.
+template <typename T> double lse_trusted(T temperature) {
+    using Limits = std::numeric_limits<T>;
+    return std::min(256.0, (double)Limits::max() * ((double)Limits::epsilon() / 8) / (double)temperature);
+}
 
 // A row's numbers in the gradient of its elements:
 //   l = (x - base) c - less, which is log p in the exponential's units,
@@ -712,11 +721,11 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
     const double lse = (double)p.lse[row_offset(p.rows, kLse, row)];
     const int64_t t = p.tokens ? p.tokens[row_offset(p.rows, kTokens, row)] : -1;
     T gp = p.g_lp ? p.g_lp[row_offset(p.rows, kGradLp, row)] : T(0);
-    const T gh = p.g_h ? p.g_h[row_offset(p.rows, kGradH, row)] : T(0);
+    T gh = p.g_h ? p.g_h[row_offset(p.rows, kGradH, row)] : T(0);
     const T h = p.g_h ? p.entropy[row_offset(p.rows, kEntropy, row)] : T(0);
-    const T gl = p.g_lse ? p.g_lse[row_offset(p.rows, kGradLse, row)] : T(0);
+    T gl = p.g_lse ? p.g_lse[row_offset(p.rows, kGradLse, row)] : T(0);
     RowGrad<T> g;
-    if (fabs(lse) <= kLseTrusted) {
+    if (fabs(lse) <= p.trusted) {
         const double b = lse * p.temperature;
         g.base = (T)b;
         g.less = (T)((b - (double)g.base) * (p.inverse * unit));
@@ -747,9 +756,12 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
     }
     if (t < 0) gp = T(0);
     if (t >= p.len) gp = T(NAN);
-    g.a = (T)((double)(gl - gp - gh * h) * p.inverse);
-    g.b = (T)((double)gh * (p.inverse / unit));
-    g.at_token = (T)((double)gp * p.inverse);
+    gp *= p.before;
+    gh *= p.before;
+    gl *= p.before;
+    g.a = (T)((double)(gl - gp - gh * h) * p.after);
+    g.b = (T)((double)gh * (p.after / unit));
+    g.at_token = (T)((double)gp * p.after);
     g.nothing = g.a * T(0);
     g.token = t >= 0 && t < p.len ? (int)t : -1;
     return g;
@@ -1165,6 +1177,12 @@ int backward_impl(kx_handle *hh, const kx_tensor *logits, const kx_tensor *token
     p.stride = logits->strides[logits->rank - 1];
     p.temperature = (double)temperature;
     p.inverse = 1.0 / (double)temperature;
+    p.trusted = lse_trusted(temperature);
+    // Gradients as large as a large temperature come out small, but their sum and
+    // the product with an entropy (21 at most) need not fit the type.  Beside 2^64
+    // nothing that the factor pushes below the normal numbers would be seen.
+    p.before = (double)temperature < 0x1p64 ? T(1) : T(1) / 64;
+    p.after = 1.0 / ((double)p.before * (double)temperature);
     p.factor = exp_factor<T>(temperature);
     DeviceGuard guard(h->device);
     if (!guard.ok) return set_err(err, KX_E_NO_DEVICE, kBwd, "cannot select device");
