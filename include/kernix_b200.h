@@ -346,7 +346,7 @@ int kx_token_log_probs_f64(kx_handle *h, const kx_tensor *logits, const kx_tenso
  * `entropy` are the forward call's for these logits and this temperature;
  * `tokens` goes with grad_log_probs.  A token below 0 takes no part of
  * grad_log_probs; one at or above the vocabulary gives its row NaN, as do NaN
- * and +inf among its logits. */
+ * and +inf among its logits, but for its logits of -inf, which keep their 0. */
 int kx_token_log_probs_backward_f32(kx_handle *h, const kx_tensor *logits, const kx_tensor *tokens,
                                     const kx_tensor *lse, const kx_tensor *entropy, const kx_tensor *grad_log_probs,
                                     const kx_tensor *grad_entropy, const kx_tensor *grad_lse, float temperature,

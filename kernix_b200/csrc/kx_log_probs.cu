@@ -751,8 +751,11 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
             st.s = ss[tid % NW];
             st.template join<NW>(p.factor, ex);
         }
-        g.base = st.m;
-        g.less = st.s == T(0) ? T(0) : (T)(log((double)st.s) * unit);
+        // a NaN or +inf in the row: NaN by way of g.a, and log p of -inf for a logit of -inf
+        const bool bad = isnan(st.s);
+        g.base = bad ? T(0) : st.m;
+        g.less = bad || st.s == T(0) ? T(0) : (T)(log((double)st.s) * unit);
+        if (bad) gl = T(NAN);
     }
     if (t < 0) gp = T(0);
     if (t >= p.len) gp = T(NAN);

@@ -26,3 +26,28 @@ def test_temperatures_near_the_largest_number(kx, torch_cuda, dtype, t, v):
         got = backward(kx, torch_cuda, x, tokens, t, *a)
         assert np.isfinite(got).all() and (got[:3] != 0).any()
         check_backward(got, x, tokens, t, dtype, *a)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("rows,v", [(9, 5), (9, 1003), (9, 5001), (3, 50_021)])
+def test_masked_logits_of_a_row_that_is_nan(kx, torch_cuda, dtype, rows, v):
+    """A NaN or +inf makes its row's gradient NaN, but for the logits of -inf,
+    whose gradient is 0 in each row; in rows aligned like their gradient and
+    not, and with a stride."""
+    torch = torch_cuda
+    x, tokens = logits(111 + v, rows, v, dtype)
+    x[:, 1::2] = -np.inf
+    x[0, 0], x[1, v - 1 - (v - 1) % 2], x[2, 2] = np.nan, np.inf, np.inf
+    gone = np.isneginf(x)
+    a = grads_in(59, rows, dtype)
+    dev = [torch.from_numpy(b).cuda() for b in a]
+    dt = torch.from_numpy(tokens).cuda()
+    wide = torch.full((rows, v + 3), 7.0, dtype=dev[0].dtype, device="cuda")
+    wide[:, 1:v + 1] = torch.from_numpy(x).cuda()
+    plain = wide[:, 1:v + 1].contiguous()
+    for view in (plain, wide[:, 1:v + 1], plain.t().contiguous().t()):
+        res = kx.token_log_probs(view, dt, entropy=True)
+        got = kx.token_log_probs_backward(view, dt, lse=res.lse, entropy=res.entropy, grad_log_probs=dev[0],
+                                          grad_entropy=dev[1], grad_lse=dev[2]).cpu().numpy()
+        assert (got[gone] == 0).all()
+        assert np.isnan(got[:3][~gone[:3]]).all() and np.isfinite(got[3:]).all()
