@@ -357,7 +357,8 @@ int kx_token_log_probs_backward_f64(kx_handle *h, const kx_tensor *logits, const
                                     const kx_tensor *grad_logits, kx_error *err);
 /* The 2-norm over all elements of `count` gradients (0 to 2^20 of them, any
  * dims and strides) into the one element of `norm`, its squares added in 64
- * bits in a fixed order.  `workspace` is the caller's device memory, 8-byte
+ * bits in a fixed order, and those of f64 elements that leave them in scaled
+ * sums: the norm is infinite only where it or an element is.  `workspace` is the caller's device memory, 8-byte
  * aligned, of at least the bytes that kx_grad_norm_workspace (host only)
  * gives; two calls that may run at the same time need one each. */
 int kx_grad_norm_workspace(uint64_t *bytes);

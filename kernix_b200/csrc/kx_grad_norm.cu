@@ -83,7 +83,37 @@ __device__ __forceinline__ void offsets(const Geom &g, I i, int64_t &so, int64_t
     d_o += (int64_t)i * g.dst[0];
 }
 
-// The same total in each thread of the block, of which this is the one call.
+// Squares are added up in 64 bits, which no square of an f32 leaves.  Those of f64
+// elements above 2^512 or below 2^-511 do, so three sums are kept: of the squares
+// as they are, of those of the elements times 2^-600 and of those times 2^600.
+// The first counts where it is finite and at least 2^-950 (what its squares lose
+// below the normal numbers is none of its 53 bits, whatever their number), the
+// second where it is infinite, the third where it is less: no square that
+// matters leaves that one.  A block whose own first sum is ordinary has the
+// second at hand and no part in the third; else it reads its elements again.
+// (All three sums in one pass took 27.8 us for 16.8 million elements, where this
+// takes 24.9 and the first sum alone 24.8.)
+template <typename T> constexpr int kSums = sizeof(T) == 4 ? 1 : 3;
+constexpr double kLarge = 0x1p-600, kSmall = 0x1p600, kLeast = 0x1p-950;
+
+// A thread's N first sums, and whether an f64 element is not zero.
+template <typename T, int N> struct Squares {
+    double s[N] = {};
+    bool any = false;
+    __device__ __forceinline__ void add(int k, T x) {
+        const double d = (double)x;
+        s[k] = fma(d, d, s[k]);
+        if constexpr (kSums<T> == 3) any = any || d != 0.0;
+    }
+    __device__ __forceinline__ double total() const {
+        double t = 0.0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) t += s[k];
+        return t;
+    }
+};
+
+// The same total in each thread of the block; a barrier lies between two calls.
 __device__ double block_total(double v) {
     constexpr int kWarps = kThreads / 32;
     __shared__ double red[kWarps];
@@ -97,20 +127,82 @@ __device__ double block_total(double v) {
     return s;
 }
 
+// The workspace: of each sum, the blocks' partial sums.
+constexpr int64_t kRoom = 16384;       // partial sums that it holds; then they are folded
+constexpr uint64_t kWorkspace = kSums<double> * kRoom * sizeof(double);
+
+// The root of all squares' sum: of the one that counts.
+template <typename T> __device__ __forceinline__ double root_of(double first, double large, double small) {
+    if (kSums<T> == 3 && first < kLeast) return sqrt(small) * (1.0 / kSmall);
+    if (kSums<T> == 3 && isinf(first)) return sqrt(large) * (1.0 / kLarge);
+    return sqrt(first);
+}
+
+// The block's partial sums from each thread's first sum; anew(by) is its sum of
+// the squares of its elements times `by`, of which any is not zero.  Their root.
+template <typename T, typename F>
+__device__ __forceinline__ double leave_partials(double mine, bool any, F anew, double *partial) {
+    const double s = block_total(mine);
+    double large = s * kLarge * kLarge, small = 0.0;
+    if constexpr (kSums<T> == 3) {
+        const bool less = s < kLeast;
+        if ((less || isinf(s)) && __syncthreads_or(any)) {
+            const double t = block_total(anew(less ? kSmall : kLarge));
+            (less ? small : large) = t;
+        }
+        if (threadIdx.x == 0) {
+            partial[kRoom + blockIdx.x] = large;
+            partial[2 * kRoom + blockIdx.x] = small;
+        }
+    }
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+    return root_of<T>(s, large, small);
+}
+
+__device__ __forceinline__ double add_partials(const double *partial, int64_t n) {
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) s += partial[i];
+    return s;
+}
+
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// A thread's sum of the squares of its block's elements times `by`, one by one:
+// rarely taken, and in few registers.
+template <typename T> __device__ __forceinline__ double chunks_anew(const Spans<T> &g, uint32_t lo, uint32_t hi, double by) {
+    double s = 0.0;
+    int k = 0;
+    for (uint32_t c = lo; c < hi; ++c) {
+        while (c >= g.first[k + 1]) ++k;
+        const Cut<T> cut(g.src[k], g.len[k]);
+        // the first chunk of a span has its edges too
+        const uint32_t part = c - g.first[k];
+        const int64_t a = cut.head + (int64_t)part * kChunk<T>, b = cut.head + cut.nv * Vec<T>::n;
+        auto add = [&](int64_t from, int64_t to) {
+#pragma unroll 1
+            for (int64_t j = from + threadIdx.x; j < to; j += kThreads) {
+                const double d = (double)g.src[k][j] * by;
+                s = fma(d, d, s);
+            }
+        };
+        add(part ? a : 0, min(a + kChunk<T>, b));
+        if (part == 0) add(b, g.len[k]);
+    }
+    return s;
+}
+
 // Sums of squares, one for each block, over its share of the chunks.  The
 // bound is the reading: 0.37 billion f32 elements take 214 us, 6.9 TB/s.  A
-// square is converted and added in 64 bits, which no f32 value can overflow,
-// and which keeps a tenth of the 64-bit pipe busy.
+// square is converted and added in 64 bits, which keeps a tenth of the 64-bit
+// pipe busy.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) sum_spans_kernel(const __grid_constant__ Spans<T> g, double *partial) {
     using V = typename Vec<T>::type;
     constexpr int VN = Vec<T>::n;
     const uint32_t lo = (uint32_t)((uint64_t)blockIdx.x * g.chunks / gridDim.x);
     const uint32_t hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * g.chunks / gridDim.x);
-    double s[VN] = {};
+    Squares<T, VN> s;
     int k = 0;
     for (uint32_t c = lo; c < hi; ++c) {
         while (c >= g.first[k + 1]) ++k;
@@ -127,26 +219,13 @@ __global__ void __launch_bounds__(kThreads) sum_spans_kernel(const __grid_consta
 #pragma unroll
         for (int u = 0; u < kVectors; ++u)
 #pragma unroll
-            for (int e = 0; e < VN; ++e) {
-                const double d = (double)reinterpret_cast<const T *>(&v[u])[e];
-                s[e] = fma(d, d, s[e]);
-            }
+            for (int e = 0; e < VN; ++e) s.add(e, reinterpret_cast<const T *>(&v[u])[e]);
         if (c == g.first[k]) {      // the span's edges
-            if ((int)threadIdx.x < cut.head) {
-                const double d = (double)x[threadIdx.x];
-                s[0] = fma(d, d, s[0]);
-            }
-            if ((int)threadIdx.x < cut.tail) {
-                const double d = (double)x[cut.head + cut.nv * VN + threadIdx.x];
-                s[0] = fma(d, d, s[0]);
-            }
+            if ((int)threadIdx.x < cut.head) s.add(0, x[threadIdx.x]);
+            if ((int)threadIdx.x < cut.tail) s.add(0, x[cut.head + cut.nv * VN + threadIdx.x]);
         }
     }
-    double t = 0.0;
-#pragma unroll
-    for (int e = 0; e < VN; ++e) t += s[e];
-    t = block_total(t);
-    if (threadIdx.x == 0) partial[blockIdx.x] = t;
+    leave_partials<T>(s.total(), s.any, [&](double by) { return chunks_anew<T>(g, lo, hi, by); }, partial);
     launch_dependents();
 }
 
@@ -155,34 +234,31 @@ __global__ void __launch_bounds__(kThreads) sum_spans_kernel(const __grid_consta
 template <typename T, typename I>
 __global__ void __launch_bounds__(kThreads) sum_strided_kernel(const T *__restrict__ x, const __grid_constant__ Geom g,
                                                                double *partial) {
-    double s = 0.0;
-    for (I i = blockIdx.x * kThreads + threadIdx.x; i < (I)g.count; i += gridDim.x * kThreads) {
-        int64_t so, d_o;
-        offsets<I>(g, i, so, d_o);
-        const double v = (double)x[so];
-        s = fma(v, v, s);
-    }
-    s = block_total(s);
-    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+    auto each = [&](auto add) {
+        for (I i = blockIdx.x * kThreads + threadIdx.x; i < (I)g.count; i += gridDim.x * kThreads) {
+            int64_t so, d_o;
+            offsets<I>(g, i, so, d_o);
+            add(x[so]);
+        }
+    };
+    Squares<T, 1> s;
+    each([&](T v) { s.add(0, v); });
+    auto anew = [&](double by) {
+        double t = 0.0;
+        each([&](T v) { t = fma((double)v * by, (double)v * by, t); });
+        return t;
+    };
+    leave_partials<T>(s.total(), s.any, anew, partial);
     launch_dependents();
 }
 
-__device__ __forceinline__ double add_partials(const double *partial, int64_t n) {
-    double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) s += partial[i];
-    return block_total(s);
-}
-
 // All partial sums by one block, in the order in which each block of the scaling
-// adds them: their root, and their sum, which may take the place of the first.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) fold_kernel(const double *partial, int64_t n, T *norm, double *total) {
+// adds them: their root, and the sums in the place of their first parts.
+template <typename T> __global__ void __launch_bounds__(kThreads) fold_kernel(double *partial, int64_t n, T *norm) {
     wait_for_previous();
-    const double s = add_partials(partial, n);
-    if (threadIdx.x == 0) {
-        *norm = (T)sqrt(s);
-        *total = s;
-    }
+    auto anew = [&](double by) { return add_partials(partial + (by == kLarge ? 1 : 2) * kRoom, n); };
+    const double root = leave_partials<T>(add_partials(partial, n), true, anew, partial);
+    if (threadIdx.x == 0) *norm = (T)root;
 }
 
 // Loads and stores of 16 bytes whose lines are the first to leave the
@@ -206,8 +282,16 @@ template <typename V> __device__ __forceinline__ void store(V *p, const V &v, ui
                  : "memory");
 }
 
-template <typename T> __device__ __forceinline__ T scale_of(double sum, double max_norm, T *norm) {
-    const double root = sqrt(sum);
+// The factor of the scaling.
+template <typename T>
+__device__ __forceinline__ T scale_of(const double *partial, int64_t n, double max_norm, T *norm) {
+    const double s = block_total(add_partials(partial, n));
+    double scaled = 0.0;
+    if (kSums<T> == 3 && (s < kLeast || isinf(s))) {
+        __syncthreads();
+        scaled = block_total(add_partials(partial + (s < kLeast ? 2 : 1) * kRoom, n));
+    }
+    const double root = root_of<T>(s, scaled, scaled);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (T)root;
     return isfinite((T)root) && root > max_norm ? (T)(max_norm / root) : T(1);
 }
@@ -226,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) scale_spans_kernel(const __grid_cons
     using V = typename Vec<T>::type;
     constexpr int VN = Vec<T>::n;
     wait_for_previous();
-    const T by = scale_of<T>(add_partials(partial, n), max_norm, norm);
+    const T by = scale_of<T>(partial, n, max_norm, norm);
     const uint32_t lo = (uint32_t)((uint64_t)blockIdx.x * g.chunks / gridDim.x);
     const uint32_t hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * g.chunks / gridDim.x);
     const uint64_t policy = SHORTLY ? leave_first() : 0;
@@ -274,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) scale_strided_kernel(const T *x, T *
                                                                  const double *partial, int64_t n, double max_norm,
                                                                  T *norm) {
     wait_for_previous();
-    const T by = scale_of<T>(add_partials(partial, n), max_norm, norm);
+    const T by = scale_of<T>(partial, n, max_norm, norm);
     for (I i = blockIdx.x * kThreads + threadIdx.x; i < (I)g.count; i += gridDim.x * kThreads) {
         int64_t so, d_o;
         offsets<I>(g, i, so, d_o);
@@ -287,7 +371,6 @@ __global__ void __launch_bounds__(kThreads) scale_strided_kernel(const T *x, T *
 // ---------------------------------------------------------------------------
 constexpr int64_t kPartials = 2048;    // most blocks of one launch over spans,
 constexpr int64_t kStrided = 512;      // over a tensor by itself
-constexpr int64_t kRoom = 16384;       // partial sums that the workspace holds; then they are folded
 constexpr uint64_t kMostTensors = 1u << 20;
 constexpr int64_t kCount32 = 1ll << 31;    // 32 bits count fewer elements, and a block's step beyond them
 constexpr int64_t kFold = 2048;        // most partial sums that each block of the scaling adds
@@ -299,8 +382,6 @@ constexpr int64_t kFold = 2048;        // most partial sums that each block of t
 // 34.7 and 33.2, 48 MB 37.1 and 37.6); of more little is left to read again (192
 // MB clipped and read: 134.9 both ways, 256 MB 179 and 176).
 constexpr int64_t kShortlyFrom = 46ll << 20, kShortlyTo = 192ll << 20;
-
-constexpr uint64_t kWorkspace = (1 + kRoom) * sizeof(double);
 
 struct Range {
     uintptr_t a, b;
@@ -514,12 +595,12 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
         s.chunks += chunks;
         s.first[++s.n] = s.chunks;
     }
-    double *total = static_cast<double *>(workspace), *partial = total + 1;
+    double *partial = static_cast<double *>(workspace);
     T *to = at<T>(norm);
     int64_t used = 0;
     auto room = [&](int64_t blocks) {   // for that many partial sums more
         if (used + blocks <= kRoom) return;
-        launch_after(h, fold_kernel<T>, 1, partial, used, to, partial);
+        launch_after(h, fold_kernel<T>, 1, partial, used, to);
         used = 1;
     };
     for (const Batch<T> &b : batches) {
@@ -539,10 +620,8 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
         ++h->launches;
         used += blocks;
     }
-    const double *sums = partial;
     if (!outs || used == 0 || used > kFold) {
-        launch_after(h, fold_kernel<T>, 1, partial, used, to, total);
-        sums = total;
+        launch_after(h, fold_kernel<T>, 1, partial, used, to);
         used = 1;
         to = nullptr;
     }
@@ -550,13 +629,13 @@ int norm_lists(Handle *h, const kx_tensor *grads, uint64_t count, double max_nor
         const bool shortly = bytes > kShortlyFrom && bytes <= kShortlyTo;
         for (const Batch<T> &b : batches) {
             launch_after(h, shortly ? scale_spans_kernel<T, true> : scale_spans_kernel<T, false>, b.blocks(h),
-                         b.spans, b.outs, sums, used, max_norm, to);
+                         b.spans, b.outs, partial, used, max_norm, to);
             to = nullptr;
         }
         for (uint64_t i : apart) {
             const Geom g = geom(&grads[i], &outs[i]);
             launch_after(h, g.count < kCount32 ? scale_strided_kernel<T, uint32_t> : scale_strided_kernel<T, int64_t>,
-                         blocks_for(g.count), at<T>(&grads[i]), at<T>(&outs[i]), g, sums, used, max_norm, to);
+                         blocks_for(g.count), at<T>(&grads[i]), at<T>(&outs[i]), g, partial, used, max_norm, to);
             to = nullptr;
         }
     }
