@@ -7,6 +7,7 @@
 // strides and the device fix, so the same gradients give the same bits again.  A norm that is not
 // finite scales nothing: the outputs are the gradients as they were.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -282,9 +283,23 @@ template <typename V> __device__ __forceinline__ void store(V *p, const V &v, ui
                  : "memory");
 }
 
-// The factor of the scaling.
+// The factor of the scaling, and 1.  A factor below the normal numbers lacks
+// digits that its products need not lack: it comes as one that has them and a
+// power of two.  The first is below 1, so that its products fit the type.
+template <typename T> struct Scale {
+    T by, then;
+    __device__ __forceinline__ T operator()(T v) const { return v * by * then; }
+};
+template <typename T> __device__ Scale<T> split_factor(double max_norm, double root) {
+    constexpr bool f32 = sizeof(T) == 4;
+    // the smallest normal power of two, or, for factors below it, the smallest of all
+    const bool last = max_norm / root < (f32 ? 0x1p-149 : 0x1p-1074);
+    const double up = f32 ? (last ? 0x1p75 : 0x1p63) : (last ? 0x1p537 : 0x1p511);
+    const double down = f32 ? (last ? 0x1p-74 : 0x1p-63) : (last ? 0x1p-537 : 0x1p-511);
+    return {(T)(max_norm * up / (root * down)), (T)(f32 ? (last ? 0x1p-149 : 0x1p-126) : (last ? 0x1p-1074 : 0x1p-1022))};
+}
 template <typename T>
-__device__ __forceinline__ T scale_of(const double *partial, int64_t n, double max_norm, T *norm) {
+__device__ __forceinline__ Scale<T> scale_of(const double *partial, int64_t n, double max_norm, T *norm) {
     const double s = block_total(add_partials(partial, n));
     double scaled = 0.0;
     if (kSums<T> == 3 && (s < kLeast || isinf(s))) {
@@ -293,7 +308,10 @@ __device__ __forceinline__ T scale_of(const double *partial, int64_t n, double m
     }
     const double root = root_of<T>(s, scaled, scaled);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (T)root;
-    return isfinite((T)root) && root > max_norm ? (T)(max_norm / root) : T(1);
+    if (!isfinite((T)root) || !(root > max_norm)) return {T(1), T(1)};
+    const T by = (T)(max_norm / root);
+    if (by < T(sizeof(T) == 4 ? FLT_MIN : DBL_MIN)) return split_factor<T>(max_norm, root);
+    return {by, T(1)};
 }
 
 // The scaled copies.  Each block adds the partial sums for itself, in one
@@ -302,15 +320,21 @@ __device__ __forceinline__ T scale_of(const double *partial, int64_t n, double m
 // room for much of the gradients (SHORTLY), neither the copies nor gradients
 // that have been read again take it from those that have not.  The bound is the
 // two streams: 0.37 billion f32 elements take 465 us, 6.3 TB/s.
+// Blocks of an SM that the registers are to leave room for (0: any number): five
+// are faster at what the cache does not hold (0.37 billion f32 elements clipped:
+// 706 us, with six 715, with four 720), the six of the other form at what it
+// does (16.8 million: 36.4, with five 36.9).
+template <bool SHORTLY> constexpr int kScaleBlocks = SHORTLY ? 0 : 5;
+
 template <typename T, bool SHORTLY>
-__global__ void __launch_bounds__(kThreads) scale_spans_kernel(const __grid_constant__ Spans<T> g,
+__global__ void __launch_bounds__(kThreads, kScaleBlocks<SHORTLY>) scale_spans_kernel(const __grid_constant__ Spans<T> g,
                                                                const __grid_constant__ Outputs<T> out,
                                                                const double *partial, int64_t n, double max_norm,
                                                                T *norm) {
     using V = typename Vec<T>::type;
     constexpr int VN = Vec<T>::n;
     wait_for_previous();
-    const T by = scale_of<T>(partial, n, max_norm, norm);
+    const Scale<T> scale = scale_of<T>(partial, n, max_norm, norm);
     const uint32_t lo = (uint32_t)((uint64_t)blockIdx.x * g.chunks / gridDim.x);
     const uint32_t hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * g.chunks / gridDim.x);
     const uint64_t policy = SHORTLY ? leave_first() : 0;
@@ -319,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) scale_spans_kernel(const __grid_cons
         while (c < g.first[k]) --k;
         const T *x = g.src[k];
         T *y = out.dst[k];
-        if (!y || (by == T(1) && x == y)) continue;     // scaled by itself, or in place already
+        if (!y || (scale.by == T(1) && x == y)) continue;     // scaled by itself, or in place already
         const Cut<T> cut(x, g.len[k]);
         const uint32_t part = c - g.first[k];
         if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0) {
@@ -334,21 +358,24 @@ __global__ void __launch_bounds__(kThreads) scale_spans_kernel(const __grid_cons
 #pragma unroll
             for (int u = 0; u < kVectors; ++u) {
 #pragma unroll
-                for (int e = 0; e < VN; ++e) reinterpret_cast<T *>(&v[u])[e] *= by;
+                for (int e = 0; e < VN; ++e) {
+                    T &each = reinterpret_cast<T *>(&v[u])[e];
+                    each = scale(each);
+                }
                 if (i0 + u * kThreads < cut.nv) {
                     if (SHORTLY) store(yv + i0 + u * kThreads, v[u], policy);
                     else yv[i0 + u * kThreads] = v[u];
                 }
             }
             if (part == 0) {
-                if ((int)threadIdx.x < cut.head) y[threadIdx.x] = x[threadIdx.x] * by;
+                if ((int)threadIdx.x < cut.head) y[threadIdx.x] = scale(x[threadIdx.x]);
                 const int64_t j = cut.head + cut.nv * VN + threadIdx.x;
-                if ((int)threadIdx.x < cut.tail) y[j] = x[j] * by;
+                if ((int)threadIdx.x < cut.tail) y[j] = scale(x[j]);
             }
         } else {    // the two lie differently against 16 bytes
             const int64_t j0 = (int64_t)part * kChunk<T>;
             const int64_t j1 = c + 1 == g.first[k + 1] ? g.len[k] : j0 + kChunk<T>;
-            for (int64_t j = j0 + threadIdx.x; j < j1; j += kThreads) y[j] = x[j] * by;
+            for (int64_t j = j0 + threadIdx.x; j < j1; j += kThreads) y[j] = scale(x[j]);
         }
     }
 }
@@ -358,11 +385,11 @@ __global__ void __launch_bounds__(kThreads) scale_strided_kernel(const T *x, T *
                                                                  const double *partial, int64_t n, double max_norm,
                                                                  T *norm) {
     wait_for_previous();
-    const T by = scale_of<T>(partial, n, max_norm, norm);
+    const Scale<T> scale = scale_of<T>(partial, n, max_norm, norm);
     for (I i = blockIdx.x * kThreads + threadIdx.x; i < (I)g.count; i += gridDim.x * kThreads) {
         int64_t so, d_o;
         offsets<I>(g, i, so, d_o);
-        out[d_o] = x[so] * by;
+        out[d_o] = scale(x[so]);
     }
 }
 

@@ -96,3 +96,36 @@ def test_f64_norms_that_no_number_holds(kx, torch_cuda):
             norm, (out,) = kx.clip_grad_norm([x], 1.0)
             assert np.isnan(norm.item()) if np.isnan(bad) else norm.item() == np.inf
             assert np.array_equal(out.cpu().numpy(), x.cpu().numpy(), equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype,size,max_norm", [
+    (np.float32, 1e12, 1e-30), (np.float32, 3e30, 1e-7), (np.float32, 1e20, 1e-37), (np.float32, 1e38, 1e-12),
+    (np.float32, 1.0, 1e-44), (np.float32, 1.0, 1e-60), (np.float64, 1e200, 1e-150), (np.float64, 3e307, 0.7),
+    (np.float64, 1e100, 1e-300), (np.float64, 1e-5, 1e-320)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_factors_below_the_normal_numbers(kx, torch_cuda, dtype, size, max_norm, apart):
+    """max_norm / norm need not be a normal number where its products are; into
+    copies, in place, at other alignments, and into outputs of other strides.
+    A result rounds once more than check_clip counts where it is itself below
+    the normal numbers: two of the smallest numbers."""
+    torch = torch_cuda
+    base = np.array([1.0, -0.75, 0.5, 1.5, -1.25, 0.3, 0.9, 1e-3, -1e-7])
+    arrs = [np.tile(base, 41).astype(dtype) * dtype(size) * dtype(0.06), (base * size).astype(dtype)]
+    dev = [torch.from_numpy(a).cuda() for a in arrs]
+    if apart:
+        dev = [torch.stack([d, torch.full_like(d, 7.0)], 1)[:, 0] for d in dev]
+    n = sum(a.size for a in arrs)
+    want = true_norm(arrs)
+    by = np.longdouble(max_norm) / want
+    u = 2.0 ** -24 if dtype == np.float32 else 2.0 ** -53
+    buf = torch.full((n + 40,), 9.0, dtype=dev[0].dtype, device="cuda")
+    odd = [buf[1:1 + arrs[0].size], buf[arrs[0].size + 11:][:arrs[1].size]]
+    norm, outs = kx.clip_grad_norm(dev, max_norm)
+    kx.clip_grad_norm_into(dev, max_norm, odd)
+    kx.clip_grad_norm_into(dev, max_norm, dev)
+    assert abs(np.longdouble(norm.item()) - want) <= want * (u + n * 2.0 ** -53)
+    for got in (outs, odd, dev):
+        for g, a in zip(got, arrs):
+            w = a.astype(np.longdouble) * by
+            tol = np.abs(w) * (3 * u + n * 2.0 ** -53) + 2 * np.longdouble(np.finfo(dtype).smallest_subnormal)
+            assert (np.abs(g.cpu().numpy().astype(np.longdouble) - w) <= tol).all()
