@@ -285,18 +285,19 @@ template <typename V> __device__ __forceinline__ void store(V *p, const V &v, ui
 
 // The factor of the scaling, and 1.  A factor below the normal numbers lacks
 // digits that its products need not lack: it comes as one that has them and a
-// power of two.  The first is below 1, so that its products fit the type.
+// power of two.  The first is 1/2 at most: its products fit the type, and it is
+// not taken for the factor 1.
 template <typename T> struct Scale {
     T by, then;
     __device__ __forceinline__ T operator()(T v) const { return v * by * then; }
 };
 template <typename T> __device__ Scale<T> split_factor(double max_norm, double root) {
     constexpr bool f32 = sizeof(T) == 4;
-    // the smallest normal power of two, or, for factors below it, the smallest of all
+    // twice the smallest normal number or, for factors below it, the smallest of all
     const bool last = max_norm / root < (f32 ? 0x1p-149 : 0x1p-1074);
-    const double up = f32 ? (last ? 0x1p75 : 0x1p63) : (last ? 0x1p537 : 0x1p511);
-    const double down = f32 ? (last ? 0x1p-74 : 0x1p-63) : (last ? 0x1p-537 : 0x1p-511);
-    return {(T)(max_norm * up / (root * down)), (T)(f32 ? (last ? 0x1p-149 : 0x1p-126) : (last ? 0x1p-1074 : 0x1p-1022))};
+    const double up = f32 ? (last ? 0x1p74 : 0x1p63) : (last ? 0x1p537 : 0x1p511);
+    const double down = f32 ? (last ? 0x1p-74 : 0x1p-62) : (last ? 0x1p-536 : 0x1p-510);
+    return {(T)(max_norm * up / (root * down)), (T)(f32 ? (last ? 0x1p-148 : 0x1p-125) : (last ? 0x1p-1073 : 0x1p-1021))};
 }
 template <typename T>
 __device__ __forceinline__ Scale<T> scale_of(const double *partial, int64_t n, double max_norm, T *norm) {

@@ -129,3 +129,12 @@ def test_factors_below_the_normal_numbers(kx, torch_cuda, dtype, size, max_norm,
             w = a.astype(np.longdouble) * by
             tol = np.abs(w) * (3 * u + n * 2.0 ** -53) + 2 * np.longdouble(np.finfo(dtype).smallest_subnormal)
             assert (np.abs(g.cpu().numpy().astype(np.longdouble) - w) <= tol).all()
+
+
+def test_a_factor_just_below_the_smallest_number_in_place(kx, torch_cuda):
+    """Its first part rounds to 1, which is not the factor 1."""
+    torch = torch_cuda
+    x = torch.zeros(9, device="cuda")
+    x[4] = 1.0
+    kx.clip_grad_norm_into([x], 2.0 ** -149 * (1 - 2.0 ** -27), [x])
+    assert x.tolist() == [0] * 4 + [2.0 ** -149] + [0] * 4
