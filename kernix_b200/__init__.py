@@ -203,15 +203,25 @@ class TensorView:
         return tuple(self.dims)
 
 
+def _refuse_pending() -> None:
+    """torch can leave a negation to a tensor's readers (``z.conj().imag``):
+    its memory does not hold its elements."""
+    raise Unsupported("a tensor with a pending negation: resolve_neg() gives its elements")
+
+
 def _descriptor(t) -> KxTensor:
     d = KxTensor()
     if isinstance(t, TensorView):
         buf = t.buffer
+        if buf.is_neg():
+            _refuse_pending()
         d.data = buf.data_ptr()
         d.storage_len = buf.numel()
         d.origin = int(t.origin)
         dims, strides = [int(n) for n in t.dims], [int(s) for s in t.strides]
     else:
+        if t.is_neg():
+            _refuse_pending()
         st = t.untyped_storage()
         d.data = st.data_ptr()
         d.storage_len = st.nbytes() // t.element_size()
@@ -240,12 +250,17 @@ def _device_index(t) -> int:
     return dev.index if dev.index is not None else 0
 
 
-def _current_stream(dev: int) -> int:
-    """torch's current stream on ``dev`` as a raw cudaStream_t (the raw query
-    when this torch build has it: no Stream object per call)."""
+@functools.lru_cache(maxsize=1)
+def _stream_query():
+    """What gives torch's current stream on a device as a raw cudaStream_t (the
+    raw query when this torch build has it: no Stream object per call)."""
     import torch
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return int(raw(dev)) if raw is not None else int(torch.cuda.current_stream(dev).cuda_stream)
+    return raw if raw is not None else lambda dev: int(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _current_stream(dev: int) -> int:
+    return _stream_query()(dev)
 
 
 def _route(t) -> Handle:
@@ -559,6 +574,8 @@ def _pack(buf, off: int, t) -> None:
     if isinstance(t, TensorView) or t.dim() > MAX_RANK:
         C.memmove(C.addressof(buf) + off, C.byref(_descriptor(t)), _SIZE)
         return
+    if t.is_neg():
+        _refuse_pending()
     shape, stride = t.shape, t.stride()
     rank = len(shape)
     if t.is_contiguous():
@@ -776,6 +793,8 @@ def _descriptors(ts, alone=()):
     words = np.frombuffer(arr, dtype=np.int64).reshape(len(ts), -1)
     views = alone and TensorView in map(type, ts)
     every = [t.buffer if isinstance(t, TensorView) else t for t in ts] if views else ts
+    if any(map(torch.Tensor.is_neg, every)):
+        _refuse_pending()
     words[:, 0] = list(map(torch.Tensor.data_ptr, every))
     words[:, 4] = words[:, 1] = list(map(torch.Tensor.numel, every))     # dims[0], storage_len
     words[:, 3] = words[:, 4 + MAX_RANK] = 1                             # rank, strides[0]
