@@ -28,6 +28,7 @@ import itertools
 import operator
 import struct
 import threading
+import warnings
 from dataclasses import dataclass, field
 from typing import NamedTuple, Sequence
 
@@ -617,12 +618,27 @@ class _Operands:
         return self.at + off
 
 
+class _General:
+    """Stands for the binding where there is none: leaves every call to the general path."""
+
+    token_log_probs = token_log_probs_backward = grad_norm = staticmethod(lambda *_: None)
+
+
 @functools.lru_cache(maxsize=1)
 def _native():
     """The binding for plain torch tensors (csrc/kx_torch.cpp); it gives None
-    for what it does not take."""
-    import torch  # noqa: F401  (the binding's symbols)
-    from . import _kx_torch
+    for what it does not take.  Without it, or with one that was built for
+    another torch, the general path takes all calls: the same kernels, but 25 us
+    on the host for a call and 69 for a list of 38 gradients and outputs."""
+    import torch
+    try:
+        from . import _kx_torch
+        if not torch.__version__.startswith(_kx_torch.torch):
+            raise ImportError(f"it was built for torch {_kx_torch.torch}, this is {torch.__version__}")
+    except ImportError as e:
+        warnings.warn(f"kernix_b200: no native binding of the calls between logits and an update "
+                      f"(python kernix_b200/_build.py builds it): {e}", RuntimeWarning, stacklevel=3)
+        return _General
     names = [f"kx_{n}_{k}" for n in ("token_log_probs", "token_log_probs_backward", "grad_norm", "clip_grad_norm")
              for k in ("f32", "f64")]
     _kx_torch.bind(*[C.cast(getattr(lib, n), C.c_void_p).value for n in (*names, "kx_grad_norm_workspace")])

@@ -3,7 +3,8 @@
 The library is self-contained (static CUDA runtime) and is written next to this
 file as ``libkernix_b200.so`` so that it travels with the source tree.  The
 binding of the Python mirror's calls on torch tensors, which knows torch and
-nothing of CUDA, is written beside it as ``_kx_torch.so``.
+nothing of CUDA, is written beside it as ``_kx_torch`` with the interpreter's
+suffix; without torch it is left out, and the C ABI is all there is.
 """
 from __future__ import annotations
 
@@ -20,7 +21,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = ROOT / "_build" / "kernix_b200"
 LIB = PKG / "libkernix_b200.so"
-BINDING = PKG / "_kx_torch.so"
+BINDING = PKG / ("_kx_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -74,11 +75,20 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 
 def _binding(force: bool, verbose: bool) -> None:
-    """Compile csrc/kx_torch.cpp against the installed torch."""
+    """Compile csrc/kx_torch.cpp against the installed torch; again where that
+    is another one than the last time, whatever its files' times."""
     src = CSRC / "kx_torch.cpp"
-    if not force and not _stale(BINDING, [src] + _headers()):
+    spec = importlib.util.find_spec("torch")
+    torch = Path(spec.submodule_search_locations[0]) if spec else None
+    if torch is None or not (torch / "include" / "ATen" / "ATen.h").exists():
+        print("kernix_b200: no torch with its headers: the Python binding is left out", file=sys.stderr)
         return
-    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    built_for, this = OBJ / "binding.txt", f"{torch}\n{(torch / 'version.py').read_text()}"
+    same = built_for.exists() and built_for.read_text() == this
+    if not force and same and not _stale(BINDING, [src] + _headers()):
+        return
+    (PKG / "_kx_torch.so").unlink(missing_ok=True)      # of any interpreter, as it was named once
+    built_for.unlink(missing_ok=True)
     tmp = BINDING.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden",
            "-I", sysconfig.get_paths()["include"], "-isystem", str(torch / "include"), "-isystem",
@@ -88,6 +98,7 @@ def _binding(force: bool, verbose: bool) -> None:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING)
+    built_for.write_text(this)
 
 
 if __name__ == "__main__":

@@ -12,6 +12,7 @@
 #include <ATen/ATen.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <vector>
 
@@ -269,4 +270,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kx_torch", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__kx_torch() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__kx_torch() {
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch", TORCH_VERSION) < 0) {     // what it was built for
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}
