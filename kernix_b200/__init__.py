@@ -655,7 +655,7 @@ def _try_native(call, t, *args):
     err = KxError()
     with h._turn:
         h.set_stream(_current_stream(dev))
-        got = call(h._h.value, dev, *args, C.addressof(err))
+        got = call(h._h.value or 0, dev, *args, C.addressof(err))
     if got is None:
         return None
     if got[0]:

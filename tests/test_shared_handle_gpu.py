@@ -50,3 +50,20 @@ def test_products_beside_log_probabilities(kx, torch_cuda):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_a_closed_handle_is_refused(kx, torch_cuda):
+    """In every call, through the binding and the general path alike."""
+    torch = torch_cuda
+    own = kx.Handle(0)
+    own.close()
+    x, t = torch.zeros(4, 4, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    view = kx.TensorView(x.reshape(-1), (4, 4), (4, 1))
+    row = torch.zeros(4, device="cuda")
+    with kx.using(own):
+        for call in (lambda: kx.matmul(x, x), lambda: kx.softmax(x, -1), lambda: kx.token_log_probs(x, t),
+                     lambda: kx.token_log_probs(view, t), lambda: kx.grad_norm([x]), lambda: kx.grad_norm([view]),
+                     lambda: kx.token_log_probs_backward(x, t, lse=row, grad_log_probs=row),
+                     lambda: kx.clip_grad_norm([x], 1.0)):
+            with pytest.raises(kx.InvalidParameter):
+                call()
