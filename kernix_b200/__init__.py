@@ -24,7 +24,6 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
-import itertools
 import operator
 import struct
 import threading
@@ -773,8 +772,8 @@ _dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape"
 
 def _lists(op: str, grads, outs=None):
     """The descriptors of a list of gradients (and of their outputs), and their
-    dtype.  Pairs of C-contiguous tensors are described by their elements
-    alone, all such pairs at once: a long list's cost is here."""
+    dtype: the lists that the binding leaves.  Pairs of C-contiguous tensors are
+    described by their elements alone, all such pairs at once."""
     import torch
     if not grads:
         raise InvalidParameter(f"{op}: grads (at least one)", operation=op, parameter="grads")
@@ -807,25 +806,15 @@ def _descriptors(ts, alone=()):
     import torch
     arr = (KxTensor * len(ts))()
     words = np.frombuffer(arr, dtype=np.int64).reshape(len(ts), -1)
-    views = alone and TensorView in map(type, ts)
-    every = [t.buffer if isinstance(t, TensorView) else t for t in ts] if views else ts
+    every = [t.buffer if isinstance(t, TensorView) else t for t in ts] if alone else ts
     if any(map(torch.Tensor.is_neg, every)):
         _refuse_pending()
     words[:, 0] = list(map(torch.Tensor.data_ptr, every))
     words[:, 4] = words[:, 1] = list(map(torch.Tensor.numel, every))     # dims[0], storage_len
     words[:, 3] = words[:, 4 + MAX_RANK] = 1                             # rank, strides[0]
-    matrices = [] if views else [i for i in alone if ts[i].dim() == 2]
-    if matrices:    # transposed weights, mostly: torch's strides are not negative, so the span starts at data_ptr
-        at, rows = [ts[i] for i in matrices], np.array(matrices)
-        dims, strides = (np.fromiter(itertools.chain.from_iterable(map(f, at)), np.int64, 2 * len(at)).reshape(-1, 2)
-                         for f in (_shape_of, torch.Tensor.stride))
-        words[rows, 1] = np.where(dims.min(1) > 0, ((dims - 1) * strides).sum(1) + 1, 0)
-        words[rows, 3] = 2
-        words[rows, 4:6], words[rows, 4 + MAX_RANK:6 + MAX_RANK] = dims, strides
-    if len(matrices) < len(alone):
-        for i in sorted({*alone} - {*matrices}):
-            words[i] = 0
-            _pack(arr, _SIZE * i, ts[i])
+    for i in alone:
+        words[i] = 0
+        _pack(arr, _SIZE * i, ts[i])
     return arr
 
 
