@@ -327,10 +327,13 @@ int kx_conv2d_backward_f64(kx_handle *h, const kx_tensor *input, const kx_tensor
  * probability -inf, and is no alternative.  Alternatives that a row does not
  * have are -inf with token -1; a row whose mask leaves nothing has an lse and
  * log probability of -inf and an entropy of 0.  A token below 0 stands for a
- * position without one: its log probability is 0.  A token at or above the
- * vocabulary gives NaN, and a row that holds a NaN or +inf gives NaN in each
- * output, with -1 for its alternatives' tokens (nothing is raised: the values
- * are never read by the host).  KX_E_PARAM names a temperature that is not
+ * position without one: its log probability is 0, in every row.  A token at or
+ * above the vocabulary gives NaN, and a row that holds a NaN or +inf gives NaN
+ * in each other output, with -1 for its alternatives' tokens (nothing is raised:
+ * the values are never read by the host).  Differences from a row's largest
+ * logit, and sums of p times them, are formed in the logits' type: at
+ * temperatures above a 21st of its largest number, where many masks of the
+ * type's lowest value still have probabilities, an entropy need not be finite.  KX_E_PARAM names a temperature that is not
  * finite and > 0 (or whose reciprocal is not), before everything else. */
 int kx_token_log_probs_f32(kx_handle *h, const kx_tensor *logits, const kx_tensor *tokens, float temperature,
                            const kx_tensor *log_probs, const kx_tensor *lse, const kx_tensor *entropy,
@@ -357,8 +360,9 @@ int kx_token_log_probs_backward_f64(kx_handle *h, const kx_tensor *logits, const
                                     const kx_tensor *grad_logits, kx_error *err);
 /* The 2-norm over all elements of `count` gradients (0 to 2^20 of them, any
  * dims and strides) into the one element of `norm`, its squares added in 64
- * bits in a fixed order, and those of f64 elements that leave them in scaled
- * sums: the norm is infinite only where it or an element is.  `workspace` is the caller's device memory, 8-byte
+ * bits, and those of f64 elements that leave them in scaled sums: the norm is
+ * infinite only where it or an element is.  The order is fixed by the sizes,
+ * strides and places against 16 bytes and by the device.  `workspace` is the caller's device memory, 8-byte
  * aligned, of at least the bytes that kx_grad_norm_workspace (host only)
  * gives; two calls that may run at the same time need one each. */
 int kx_grad_norm_workspace(uint64_t *bytes);

@@ -464,6 +464,8 @@ class CudaExecutor {
     }
     // The 2-norm over all elements of a list of gradients, and the list scaled
     // in place to a norm of at most max_norm (kx_grad_norm_*, kx_clip_grad_norm_*).
+    // Both allocate a workspace for the call and wait for its end, so they are not
+    // for capture into a graph, as the C entries are.
     template <typename T>
     DeviceTensor<T> grad_norm(const std::vector<DeviceTensor<T>> &grads) const {
         return norm_of<T>(grads, nullptr);

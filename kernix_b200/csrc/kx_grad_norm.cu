@@ -3,9 +3,11 @@
 //
 //   norm = sqrt(sum over all tensors of g^2),  out = g * min(1, max_norm / norm)
 //
-// Squares are added in 64 bits in an order that only the gradients' sizes and
-// strides and the device fix, so the same gradients give the same bits again.  A norm that is not
-// finite scales nothing: the outputs are the gradients as they were.
+// Squares are added in 64 bits in an order that the gradients' sizes, strides
+// and places against 16 bytes and the device fix: the same gradients where they
+// were give the same bits again, and elsewhere bits that may differ in the last
+// place of the sum.  A norm that is not finite scales nothing: the outputs are
+// the gradients as they were.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -408,7 +410,8 @@ constexpr int64_t kFold = 2048;        // most partial sums that each block of t
 // 64 MB in 32.5 and 35.3, 128 MB in 62.0 and 65.6.  Fewer have room beside their
 // copies, which are there for who reads them next (clipped and read, 44 MB take
 // 34.7 and 33.2, 48 MB 37.1 and 37.6); of more little is left to read again (192
-// MB clipped and read: 134.9 both ways, 256 MB 179 and 176).
+// MB clipped and read: 134.9 both ways, 256 MB 179 and 176).  All of that is of
+// copies apart; lists clipped in place follow the same rule, unmeasured.
 constexpr int64_t kShortlyFrom = 46ll << 20, kShortlyTo = 192ll << 20;
 
 struct Range {

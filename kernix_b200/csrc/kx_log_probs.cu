@@ -344,10 +344,12 @@ constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 && 
 // then in shared memory, then (few rows) in that of the cluster's first block,
 // so that one launch and no workspace do for any number of rows.  The bound is
 // the reading of the logits: 4096 x 32000 f32 with entropies takes 80 us, 6.5
-// TB/s; in f64 it is arithmetic, 48 instructions for an element of which the
-// 64-bit pipe takes 17: 509 x 32003 takes 45 us.  (Copies into shared memory two
-// steps ahead, with half as many elements of a thread at a time, took 61: what
-// keeps the pipe busy is the number of independent exponentials.)  Few rows wait
+// TB/s.  In f64 an element takes 48 instructions, 17 of them of the 64-bit pipe,
+// and 509 x 32003 with 4 alternatives 49 us: a third of the warps' places are
+// taken, which leaves that pipe 46 % and the issue 57 % busy, and some SMs have
+// four rows where the mean is 3.4.  (Copies into shared memory two steps ahead,
+// with half as many elements of a thread at a time, took 61 us where this took
+// 52: it is the number of independent exponentials that counts.)  Few rows wait
 // for one memory round trip after another: 1 x 32000 f32 takes 3.7 us, with
 // alternatives 5.8 to 6.4.
 //
@@ -357,8 +359,12 @@ constexpr int kBlocks = NW == 1 ? (sizeof(T) == 4 ? 9 : 5) : (sizeof(T) == 4 && 
 // of theirs again whose own maxima do, about 4 % of the row: going over all of
 // their elements took 97 us where this took 72, and takes 63 now (1501 x 50021
 // f32, 8 alternatives, half of the tokens masked).  A few dozen candidates are ranked
-// by counting.  Should more than kCandidates elements reach the bound (rows of
-// equal values), the alternatives are found one after another instead.
+// by counting.  Should more than kCandidates elements reach the bound, the
+// alternatives are found one after another instead, with a reading of the
+// block's part for each: rows of equal values (64 x 32000 f32 with 8: 27 us for
+// 7.5; 300 x 32000 with 20: 236 for 14.7; 1501 x 50021 with 8: 803 for 59), and
+// rows of which a mask leaves one run so short that some warp has none of it and
+// yet longer than kCandidates (700 tokens: 24, 224 and 58 us).
 template <typename T, bool VEC, bool ENT, int NW, bool WIDE = false>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
     log_probs_kernel(const __grid_constant__ ForwardParams<T> p) {
@@ -500,9 +506,9 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, kBlocks<T, NW, WIDE>)
             if (n <= kCandidates<NW>) {
                 for (int k = n + tid; k < p.top; k += GT) sh.best[k] = Key<T>::none(32 * rank + k);
                 // Four lanes for each candidate where a row has eight warps (509
-                // x 32003 f64, 4 alternatives: 44.8 us, one lane 46.8; four warps
-                // have rows enough to wait for, and 85.7 us for the 79.6 of 4096
-                // x 32000 f32 with the code of it in their kernel).
+                // x 32003 f64, 4 alternatives: 49.2 us, one lane 50.7); four warps
+                // have rows enough to wait for (4096 x 32000 f32: 80.6 us, with
+                // the code of it in their kernel 80.8).
                 constexpr int kLanes = NW == 8 ? 4 : 1;
                 for (int k0 = tid / 32 * (32 / kLanes); k0 < n; k0 += GT / kLanes) {
                     const int k = k0 + lane / kLanes;
@@ -771,8 +777,12 @@ __device__ __forceinline__ RowGrad<T> row_grad(const BackwardParams<T> &p, int64
 }
 
 // The gradient: one element in, one out, with a row's few numbers between
-// them.  The bound is the two streams: 4096 x 32000 f32 takes 165 us, 6.4
-// TB/s, and 169 where the two lie differently against 16 bytes.  A block takes a
+// them.  The bound is the two streams: 4096 x 32000 f32 takes 164 us, 6.4
+// TB/s, and 169 where the two lie differently against 16 bytes.  A row that is
+// taken anew is read once more by each of its parts: with lse = 600, at T =
+// 0.05, the same takes 218 us, 8 x 131072 19.1 us for 3.8 and 1 x 131072 15.7 for
+// 3.4.  At 64 registers a thread the f64 forms spill 56 to 132 bytes, the f32
+// forms 32 at most.  A block takes a
 // part of one row: parts of 32000 elements there, where parts of 8192 took 190 us
 // and of 2048 343, as each begins with its row's numbers; or each of its warps a
 // short row (4096 x 1000: 8 us, with a block for each row 23).
