@@ -165,14 +165,14 @@ def handle(device: int | None = None) -> Handle:
     default).  Threads may share it: each call binds the thread's current
     stream and enqueues in one turn.  Its scratch (split sums, gathered
     operands) is one buffer, so products that run at the same time on several
-    streams want a handle each (``using``)."""
+    streams want a handle each (``using``).  The first call makes it, which a
+    stream that is being captured does not allow: make it before."""
     import torch
     if device is None:
         device = torch.cuda.current_device()
     h = _handles.get(device)
     if h is None:
-        h = Handle(device)
-        _handles[device] = h
+        h = _handles.setdefault(device, Handle(device))     # the first of threads that ask at once
     return h
 
 

@@ -186,3 +186,22 @@ def test_a_finaliser_may_call_within_a_turn():
     assert h._turn.acquire(timeout=1) and h._turn.acquire(timeout=1)
     h._turn.release()
     h._turn.release()
+
+
+def test_threads_that_make_the_first_handle_at_once_share_it(monkeypatch):
+    """Else each would have a turn, and calls of both, of its own."""
+    both = threading.Barrier(2, timeout=5)
+
+    class Slow:
+        def __init__(self, device):
+            both.wait()
+
+    monkeypatch.setattr(kx, "Handle", Slow)
+    monkeypatch.setattr(kx, "_handles", {})
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(kx.handle(3))) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(10)
+    assert len(got) == 2 and got[0] is got[1] is kx.handle(3)
