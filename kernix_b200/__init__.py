@@ -348,30 +348,24 @@ def matmul_into_replicated(a, b, out, out_mc: int) -> None:
     _enqueue(h, fn, C.byref(da), C.byref(db), C.byref(do), C.c_void_p(base))
 
 
-class _Ordered:
+@contextlib.contextmanager
+def _ordered(h: Handle):
     """Run the enclosed device calls of ``h`` in ordered mode, in one turn of
     the handle: other threads' calls keep their own mode."""
-
-    def __init__(self, h: Handle):
-        self.h = h
-
-    def __enter__(self):
-        self.h._turn.acquire()
-        self.prev = self.h.ordered_matmul
-        self.h.set_ordered_matmul(True)
-        return self.h
-
-    def __exit__(self, *exc):
-        self.h.set_ordered_matmul(self.prev)
-        self.h._turn.release()
-        return False
+    with h._turn:
+        before = h.ordered_matmul
+        h.set_ordered_matmul(True)
+        try:
+            yield
+        finally:
+            h.set_ordered_matmul(before)
 
 
 def matmul_reference(a, b):
     """``matmul_reference`` on the device: every output accumulated in
     increasing k with separately rounded multiply and add (linalg.rs:57-64),
     so the bits equal Kernix's ordered CPU result."""
-    with _Ordered(_route(a)):
+    with _ordered(_route(a)):
         return matmul(a, b)
 
 
@@ -428,7 +422,7 @@ def conv2d_into(x, w, out, options: Conv2dOptions = Conv2dOptions()) -> None:
 def conv2d_reference(x, w, options: Conv2dOptions = Conv2dOptions()):
     """``conv2d_reference`` on the device: the ordered scalar loop
     (neural.rs:188-198, 341-357), bitwise equal to Kernix's CPU result."""
-    with _Ordered(_route(x)):
+    with _ordered(_route(x)):
         return conv2d(x, w, options)
 
 

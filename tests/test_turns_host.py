@@ -205,3 +205,27 @@ def test_threads_that_make_the_first_handle_at_once_share_it(monkeypatch):
     for t in threads:
         t.join(10)
     assert len(got) == 2 and got[0] is got[1] is kx.handle(3)
+
+
+@pytest.mark.parametrize("name", ["matmul", "matmul_reference", "conv2d_reference", "token_log_probs", "grad_norm"])
+def test_a_call_that_fails_gives_the_turn_back(shared, name):
+    def fails(*_):
+        raise kx.InvalidParameter("no")
+
+    for broken in ("set_stream", "set_ordered_matmul"):
+        if broken == "set_ordered_matmul" and "reference" not in name:
+            continue
+        setattr(shared.h, broken, fails)
+        threading.current_thread().name, mine = "second", threading.current_thread().name
+        try:
+            with pytest.raises(kx.InvalidParameter):
+                operators()[name]()
+        finally:
+            threading.current_thread().name = mine
+        delattr(shared.h, broken)
+        free = []
+        t = threading.Thread(target=lambda: free.append(shared.h._turn.acquire(timeout=2)))
+        t.start()
+        t.join()
+        assert free == [True]
+        shared.h._turn = threading.RLock()
