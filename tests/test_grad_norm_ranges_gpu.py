@@ -138,3 +138,26 @@ def test_a_factor_just_below_the_smallest_number_in_place(kx, torch_cuda):
     x[4] = 1.0
     kx.clip_grad_norm_into([x], 2.0 ** -149 * (1 - 2.0 ** -27), [x])
     assert x.tolist() == [0] * 4 + [2.0 ** -149] + [0] * 4
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_the_order_of_the_sums(kx, torch_cuda, dtype):
+    """The same values at the same places against 16 bytes have the same bits,
+    wherever they are; at other places the sums' order is another, and the norm
+    within the bounds of any order."""
+    torch = torch_cuda
+    ty = torch.float32 if dtype == np.float32 else torch.float64
+    n, size = 30_011, torch.tensor([], dtype=ty).element_size()
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(n, generator=gen, device="cuda", dtype=ty)
+    want = true_norm([x.cpu().numpy()])
+    u = 2.0 ** -24 if dtype == np.float32 else 2.0 ** -53
+    buf = torch.empty(8 * (n + 64), device="cuda", dtype=ty)
+    seen = {}
+    for start in (0, 4, 64, 1, 5, 17, 2, 3, 7):
+        at = buf[start:start + n]
+        at.copy_(x)
+        norm = kx.grad_norm([at]).item()
+        assert abs(np.longdouble(norm) - want) <= want * (u + n * 2.0 ** -53)
+        assert seen.setdefault(at.data_ptr() % 16, norm) == norm
+    assert len(seen) == 16 // size
